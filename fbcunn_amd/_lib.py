@@ -15,6 +15,7 @@ LIB_PATH = os.path.join(_HERE, "libfbfftconv.so")
 
 OK, ERR_INVALID_ARGUMENT, ERR_UNSUPPORTED_SIZE, ERR_UNSUPPORTED_DIMENSION, ERR_OUT_OF_MEMORY, ERR_HIP = range(6)
 REUSE_NONE, REUSE_INPUT, REUSE_OUTPUT, REUSE_WEIGHT, REUSE_ALL = 0, 1, 2, 4, 7
+F32, BF16, F16 = 0, 1, 2
 STAGE_NAMES = ("fft_a", "fft_b", "mm", "ifft", "bias_grad")
 
 
@@ -38,6 +39,15 @@ class PlanInfo(ctypes.Structure):
                 ("output_freq_bytes", ctypes.c_size_t), ("scratch_bytes", ctypes.c_size_t),
                 ("tiles_h", ctypes.c_int), ("tiles_w", ctypes.c_int),
                 ("backward_freq_bytes", ctypes.c_size_t)]
+
+
+class AdamwConfig(ctypes.Structure):
+    _fields_ = [("param_type", ctypes.c_int), ("grad_type", ctypes.c_int), ("state_bits", ctypes.c_int),
+                ("seed", ctypes.c_uint), ("beta1", ctypes.c_double), ("beta2", ctypes.c_double), ("eps", ctypes.c_double)]
+
+
+class AdamwTensor(ctypes.Structure):
+    _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("n", ctypes.c_long)]
 
 
 _vp, _i, _f, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long
@@ -84,6 +94,13 @@ SIGNATURES = {
     "fbfc_bias_grad_scratch_bytes": (ctypes.c_size_t, [_i, _i]),
     "fbfc_acc_grad_parameters_bias": (_i, [_vp, _vp, _f, _i, _i, _i, _i, _vp, _vp]),
     "fbfc_acc_grad_parameters_bias_noalloc": (_i, [_vp, _vp, _f, _i, _i, _i, _i, _vp]),
+    "fbfc_adamw_state_elements": (_l, [ctypes.POINTER(AdamwTensor), _i]),
+    "fbfc_adamw_create": (_i, [ctypes.POINTER(AdamwConfig), ctypes.POINTER(AdamwTensor), _i, _vp, _vp, _vp, _vp,
+                               ctypes.POINTER(_vp)]),
+    "fbfc_adamw_destroy": (_i, [_vp]),
+    "fbfc_adamw_step": (_i, [_vp, ctypes.c_double, ctypes.c_double, _f, _vp]),
+    "fbfc_adamw_set_step": (_i, [_vp, _l, _vp]),
+    "fbfc_adamw_get_step": (_i, [_vp, ctypes.POINTER(_l), _vp]),
 }
 
 _lib = None

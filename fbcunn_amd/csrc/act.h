@@ -1,0 +1,58 @@
+// Activations in 32, 16 (bfloat16) or 16 (half) bits: vectors of them in memory, numbers of 32 bits in registers.
+// Every conversion to fewer bits rounds to the nearest, ties to even.
+#pragma once
+#include <hip/hip_runtime.h>
+
+namespace fbfc {
+
+enum ActType { kF32 = 0, kBF16 = 1, kF16 = 2 };  // the values of FBFC_F32, FBFC_BF16, FBFC_F16
+
+using bf16 = __bf16;
+using f16 = _Float16;
+
+// N consecutive values.  The alignment is that of one value: rows of odd length and views into a flattened storage
+// begin anywhere, and gfx950 reads and writes global memory in vectors of up to 16 bytes at any address, so one
+// path serves all of them.
+template <typename T, int N>
+struct VecOf {
+    typedef T type __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+};
+template <typename T, int N>
+using Vec = typename VecOf<T, N>::type;
+
+// Always global memory, which the compiler cannot tell of an address that was itself read from memory.
+#define FBFC_GLOBAL __attribute__((address_space(1)))
+template <int N, typename T>
+__device__ __forceinline__ Vec<T, N> load_vec(const T *p)
+{
+    return *(const FBFC_GLOBAL Vec<T, N> *)(p);
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_vec(T *p, Vec<T, N> v)
+{
+    *(FBFC_GLOBAL Vec<T, N> *)(p) = v;
+}
+
+// The first `n` of N values, the others zero; what lies behind them is not touched.
+template <int N, typename T>
+__device__ __forceinline__ Vec<T, N> load_some(const T *p, long n)
+{
+    if (n >= N) return load_vec<N>(p);
+    Vec<T, N> v;
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = i < n ? ((const FBFC_GLOBAL T *)p)[i] : (T)0.0f;
+    return v;
+}
+template <int N, typename T>
+__device__ __forceinline__ void store_some(T *p, Vec<T, N> v, long n)
+{
+    if (n >= N) {
+        store_vec<N>(p, v);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+        if (i < n) ((FBFC_GLOBAL T *)p)[i] = v[i];
+}
+
+}  // namespace fbfc

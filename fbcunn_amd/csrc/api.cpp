@@ -12,6 +12,7 @@
 #include <string>
 
 #include "../../include/fbfftconv.h"
+#include "errors.h"
 #include "kernels.h"
 
 namespace fbfc {
@@ -43,11 +44,7 @@ bool launch_events_next(hipEvent_t *start, hipEvent_t *stop)
     return true;
 }
 
-}  // namespace fbfc
-
-namespace {
-
-thread_local std::string g_last_error;
+static thread_local std::string g_last_error;
 
 int fail(int code, const std::string &msg)
 {
@@ -59,6 +56,13 @@ int fail_hip(hipError_t e, const char *what)
 {
     return fail(FBFC_ERR_HIP, std::string(what) + ": " + hipGetErrorString(e));
 }
+
+}  // namespace fbfc
+
+using fbfc::fail;
+using fbfc::fail_hip;
+
+namespace {
 
 constexpr int kMinFft = 8;
 constexpr int kMaxFft = 128;
@@ -309,12 +313,6 @@ struct StageTimer {
     }
 };
 
-#define FBFC_TRY(expr, what)                                   \
-    do {                                                       \
-        hipError_t e_ = (expr);                                \
-        if (e_ != hipSuccess) return fail_hip(e_, what);       \
-    } while (0)
-
 // A stage of a pass: launched once, or tm.reps() times back to back when the plan is timed
 // (every stage is a pure function of its inputs, so repeating it changes no result).
 #define FBFC_STAGE(tm, expr, what)                             \
@@ -393,7 +391,7 @@ extern "C" {
 
 const char *fbfc_version(void) { return "fbfftconv 0.1 (gfx950)"; }
 
-const char *fbfc_last_error(void) { return g_last_error.c_str(); }
+const char *fbfc_last_error(void) { return fbfc::g_last_error.c_str(); }
 
 const char *fbfc_last_launch(void) { return fbfc::kernel_log_get(); }
 

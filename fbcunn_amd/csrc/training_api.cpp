@@ -1,0 +1,241 @@
+// C ABI of the training and serving operators: argument checking and launches.  Every argument is checked before the
+// first call of the HIP runtime, so refusals need no GPU.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <cstdio>
+#include <new>
+#include <vector>
+
+#include "../../include/fbfftconv.h"
+#include "errors.h"
+#include "kernels.h"
+#include "training.h"
+
+using fbfc::fail;
+
+static_assert(FBFC_F32 == fbfc::kF32 && FBFC_BF16 == fbfc::kBF16 && FBFC_F16 == fbfc::kF16, "one set of values");
+
+namespace {
+
+bool type_ok(int t) { return t == FBFC_F32 || t == FBFC_BF16 || t == FBFC_F16; }
+size_t type_bytes(int t) { return t == FBFC_F32 ? 4 : 2; }
+bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
+
+// A stretch of memory that a call reads or writes.
+struct Range {
+    uintptr_t begin, end;
+    bool written;
+};
+
+// Whether something that is written shares memory with anything else.
+bool ranges_overlap(std::vector<Range> &r)
+{
+    std::sort(r.begin(), r.end(), [](const Range &a, const Range &b) { return a.begin < b.begin; });
+    uintptr_t any = 0, written = 0;
+    for (const Range &x : r) {
+        if (x.begin == x.end) continue;
+        if (x.begin < (x.written ? any : written)) return true;
+        any = std::max(any, x.end);
+        if (x.written) written = std::max(written, x.end);
+    }
+    return false;
+}
+
+}  // namespace
+
+struct fbfc_adamw {
+    int device;
+    fbfc_adamw_config config;
+    void *memory;  // the clock, then the table of pieces
+    fbfc::AdamwArgs args;
+};
+
+extern "C" {
+
+// ---- AdamW ---------------------------------------------------------------------------------------
+long fbfc_adamw_state_elements(const fbfc_adamw_tensor *tensors, int count)
+{
+    if (tensors == nullptr || count < 1) return 0;
+    long n = 0;
+    for (int i = 0; i < count; ++i) {
+        if (tensors[i].n < 0 || tensors[i].n > (1L << 40)) return 0;
+        n += (tensors[i].n + fbfc::kAdamwBlock - 1) / fbfc::kAdamwBlock * fbfc::kAdamwBlock;
+    }
+    return n;
+}
+
+static int adamw_check(const fbfc_adamw_config *c, const fbfc_adamw_tensor *tensors, int count, const void *m,
+                       const void *v, const float *m_scale, const float *v_scale)
+{
+    if (c == nullptr || tensors == nullptr || m == nullptr || v == nullptr)
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    if (count < 1) return fail(FBFC_ERR_INVALID_ARGUMENT, "at least one tensor is needed");
+    if (!type_ok(c->param_type) || !type_ok(c->grad_type)) return fail(FBFC_ERR_INVALID_ARGUMENT, "unknown type");
+    if (c->state_bits != 8 && c->state_bits != 32)
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "states have 8 or 32 bits");
+    if (!(c->beta1 >= 0 && c->beta1 < 1 && c->beta2 >= 0 && c->beta2 < 1))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "betas must be in [0, 1)");
+    if (!(c->eps > 0 && std::isfinite(c->eps) && (float)c->eps > 0.0f))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "eps must be positive");
+    if (c->state_bits == 8 && (m_scale == nullptr || v_scale == nullptr))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "states of 8 bits need their scales");
+    if (!aligned(m, 16) || !aligned(v, 16)) return fail(FBFC_ERR_INVALID_ARGUMENT, "states must be 16-byte aligned");
+    if (c->state_bits == 8 && (!aligned(m_scale, 4) || !aligned(v_scale, 4)))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "scales must be 4-byte aligned");
+    const size_t pb = type_bytes(c->param_type), gb = type_bytes(c->grad_type), sb = c->state_bits / 8;
+    long pieces = 0;
+    for (int i = 0; i < count; ++i) {
+        const fbfc_adamw_tensor &t = tensors[i];
+        if (t.n < 0) return fail(FBFC_ERR_INVALID_ARGUMENT, "sizes must not be negative");
+        if (t.n > (1L << 40)) return fail(FBFC_ERR_UNSUPPORTED_SIZE, "a tensor of more than 2^40 parameters");
+        if (t.n > 0 && (t.param == nullptr || t.grad == nullptr)) return fail(FBFC_ERR_INVALID_ARGUMENT, "null tensor");
+        if (!aligned(t.param, pb) || !aligned(t.grad, gb))
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "tensors must be aligned to their type");
+        pieces += (t.n + fbfc::kAdamwPiece - 1) / fbfc::kAdamwPiece;
+    }
+    if (pieces > INT32_MAX) return fail(FBFC_ERR_UNSUPPORTED_SIZE, "too many parameters for one optimizer");
+    const size_t n = (size_t)fbfc_adamw_state_elements(tensors, count);
+    std::vector<Range> r;
+    r.reserve(2 * (size_t)count + 4);
+    auto add = [&r](const void *p, size_t bytes, bool written) {
+        r.push_back({reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes, written});
+    };
+    for (int i = 0; i < count; ++i) {
+        add(tensors[i].param, tensors[i].n * pb, true);
+        add(tensors[i].grad, tensors[i].n * gb, false);
+    }
+    add(m, n * sb, true);
+    add(v, n * sb, true);
+    if (c->state_bits == 8) {
+        add(m_scale, n / fbfc::kAdamwBlock * 4, true);
+        add(v_scale, n / fbfc::kAdamwBlock * 4, true);
+    }
+    if (ranges_overlap(r))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "a parameter or a state shares memory with another tensor");
+    return FBFC_OK;
+}
+
+static int adamw_create(const fbfc_adamw_config *c, const fbfc_adamw_tensor *tensors, int count, void *m, void *v,
+                        float *m_scale, float *v_scale, fbfc_adamw **out)
+{
+    const int rc = adamw_check(c, tensors, count, m, v, m_scale, v_scale);
+    if (rc != FBFC_OK) return rc;
+    std::vector<fbfc::AdamwPiece> pieces;
+    const size_t pb = type_bytes(c->param_type), gb = type_bytes(c->grad_type);
+    long first = 0;
+    for (int i = 0; i < count; ++i) {
+        const fbfc_adamw_tensor &t = tensors[i];
+        for (long o = 0; o < t.n; o += fbfc::kAdamwPiece)
+            pieces.push_back({static_cast<char *>(t.param) + o * pb, static_cast<const char *>(t.grad) + o * gb, first + o,
+                              std::min<long>(t.n - o, fbfc::kAdamwPiece)});
+        first += (t.n + fbfc::kAdamwBlock - 1) / fbfc::kAdamwBlock * fbfc::kAdamwBlock;
+    }
+    fbfc_adamw *p = new (std::nothrow) fbfc_adamw();
+    if (p == nullptr) return fail(FBFC_ERR_OUT_OF_MEMORY, "host allocation failed");
+    p->config = *c;
+    constexpr size_t head = 256;
+    static_assert(sizeof(fbfc::AdamwClock) <= head, "the clock has a line of its own");
+    const fbfc::AdamwClock clock = fbfc::adamw_clock(0, c->beta1, c->beta2, c->seed);
+    hipError_t e = hipGetDevice(&p->device);
+    if (e == hipSuccess) e = hipMalloc(&p->memory, head + pieces.size() * sizeof(fbfc::AdamwPiece));
+    if (e == hipSuccess) e = hipMemcpy(p->memory, &clock, sizeof clock, hipMemcpyHostToDevice);
+    if (e == hipSuccess && !pieces.empty())
+        e = hipMemcpy(static_cast<char *>(p->memory) + head, pieces.data(), pieces.size() * sizeof(fbfc::AdamwPiece),
+                      hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        (void)hipGetLastError();
+        fbfc_adamw_destroy(p);
+        if (e == hipErrorOutOfMemory) return fail(FBFC_ERR_OUT_OF_MEMORY, "no memory for the optimizer's table");
+        return fbfc::fail_hip(e, "optimizer allocation");
+    }
+    fbfc::AdamwArgs &a = p->args;
+    a.pieces = reinterpret_cast<const fbfc::AdamwPiece *>(static_cast<char *>(p->memory) + head);
+    a.n_pieces = (int)pieces.size();
+    a.clock = static_cast<fbfc::AdamwClock *>(p->memory);
+    a.m = m;
+    a.v = v;
+    a.m_scale = m_scale;
+    a.v_scale = v_scale;
+    a.beta1 = c->beta1;
+    a.beta2 = c->beta2;
+    a.seed = c->seed;
+    a.keep1 = (float)c->beta1;
+    a.take1 = (float)(1 - c->beta1);
+    a.keep2 = (float)c->beta2;
+    a.take2 = (float)(1 - c->beta2);
+    a.eps = (float)c->eps;
+    *out = p;
+    return FBFC_OK;
+}
+
+int fbfc_adamw_create(const fbfc_adamw_config *config, const fbfc_adamw_tensor *tensors, int count, void *m, void *v,
+                      float *m_scale, float *v_scale, fbfc_adamw **opt)
+{
+    if (opt == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    *opt = nullptr;
+    try {
+        return adamw_create(config, tensors, count, m, v, m_scale, v_scale, opt);
+    } catch (const std::bad_alloc &) {
+        return fail(FBFC_ERR_OUT_OF_MEMORY, "host allocation failed");
+    }
+}
+
+int fbfc_adamw_destroy(fbfc_adamw *p)
+{
+    if (p == nullptr) return FBFC_OK;
+    if (p->memory) (void)hipFree(p->memory);
+    delete p;
+    return FBFC_OK;
+}
+
+static int adamw_device(const fbfc_adamw *p)
+{
+    int device = -1;
+    FBFC_TRY(hipGetDevice(&device), "hipGetDevice");
+    if (device != p->device)
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "the optimizer was made on another device than the current one");
+    return FBFC_OK;
+}
+
+int fbfc_adamw_set_step(fbfc_adamw *p, long t, void *stream)
+{
+    if (p == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    if (t < 0) return fail(FBFC_ERR_INVALID_ARGUMENT, "the number of steps must not be negative");
+    const int rc = adamw_device(p);
+    if (rc != FBFC_OK) return rc;
+    FBFC_TRY(fbfc::launch_adamw_set_clock(p->args, t, static_cast<hipStream_t>(stream)), "AdamW clock");
+    return FBFC_OK;
+}
+
+int fbfc_adamw_get_step(fbfc_adamw *p, long *t, void *stream)
+{
+    if (p == nullptr || t == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    const int rc = adamw_device(p);
+    if (rc != FBFC_OK) return rc;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    FBFC_TRY(hipMemcpyAsync(t, &p->args.clock->t, sizeof *t, hipMemcpyDeviceToHost, s), "AdamW step count");
+    FBFC_TRY(hipStreamSynchronize(s), "hipStreamSynchronize");
+    return FBFC_OK;
+}
+
+int fbfc_adamw_step(fbfc_adamw *p, double lr, double weight_decay, float grad_scale, void *stream)
+{
+    if (p == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    if (!std::isfinite(lr) || !std::isfinite(weight_decay))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "the learning rate and the weight decay must be finite");
+    const int rc = adamw_device(p);
+    if (rc != FBFC_OK) return rc;
+    fbfc::kernel_log_clear();
+    fbfc::AdamwArgs a = p->args;
+    a.lr = lr;
+    a.decay = (float)(1 - lr * weight_decay);
+    a.grad_scale = grad_scale;
+    FBFC_TRY(fbfc::launch_adamw(p->config.param_type, p->config.grad_type, p->config.state_bits, a,
+                                static_cast<hipStream_t>(stream)), "AdamW step");
+    return FBFC_OK;
+}
+
+}  // extern "C"

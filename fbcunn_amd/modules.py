@@ -14,29 +14,11 @@ import torch
 
 from . import _lib
 from ._lib import ConvDesc, FbfcError, PlanInfo, check, lib
+from .tensors import _check_tensor, _ptr, _stream
 
 __all__ = ["SpatialConvolutionFFT", "SpatialConvolutionFBFFT", "SpatialConvolutionFBFFTGemm", "SpatialConvolutionDirect",
            "SpatialConvolutionFFTTiled", "SpatialConvolutionFFTTiledSync", "SpatialConvolutionFFTTiledAsync",
            "SpatialConvolutionFFTTiledIterated", "FFTWrapper", "transposeMM", "updateOutputBias", "accGradParametersBias", "FbfcError"]
-
-
-def _ptr(t):
-    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
-
-
-def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
-
-
-def _check_tensor(t, name, ndim=None, strided=False):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda:
-        raise TypeError("%s: CUDA support only!" % name)   # the reference's assert message
-    if t.dtype != torch.float32:
-        raise TypeError("%s must be float32" % name)
-    if ndim is not None and t.dim() != ndim:
-        raise ValueError("%s must be %d-D" % (name, ndim))
-    if not strided and not t.is_contiguous():
-        raise ValueError("%s must be contiguous" % name)
 
 
 class _Plan:

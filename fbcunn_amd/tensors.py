@@ -1,0 +1,27 @@
+"""What the modules share to hand torch tensors to the C ABI: addresses, the current stream, checks."""
+import ctypes
+
+import torch
+
+from . import _lib
+
+TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _ptr(t):
+    return ctypes.c_void_p(t.data_ptr()) if t is not None else ctypes.c_void_p(0)
+
+
+def _stream():
+    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+
+
+def _check_tensor(t, name, ndim=None, strided=False):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise TypeError("%s: CUDA support only!" % name)   # the reference's assert message
+    if t.dtype != torch.float32:
+        raise TypeError("%s must be float32" % name)
+    if ndim is not None and t.dim() != ndim:
+        raise ValueError("%s must be %d-D" % (name, ndim))
+    if not strided and not t.is_contiguous():
+        raise ValueError("%s must be contiguous" % name)

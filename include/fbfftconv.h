@@ -339,6 +339,53 @@ int fbfc_acc_grad_parameters_bias_strided(const float *grad_output, float *grad_
 int fbfc_acc_grad_parameters_bias_noalloc(const float *grad_output, float *grad_bias, float scale,
                                           int batch, int planes, int h, int w, void *stream);
 
+/* Training and serving operators ---------------------------------------------------
+ * What a network around the convolution layers needs besides them.  None has a counterpart in the
+ * reference.  Activations may have 32 or 16 bits; parameters of the layers, their gradients and every
+ * sum have 32. */
+enum { FBFC_F32 = 0, FBFC_BF16 = 1, FBFC_F16 = 2 };
+
+/* One AdamW step over all the parameters of a network, in one launch:
+ *     g' = grad_scale g        m = beta1 m + (1 - beta1) g'        v = beta2 v + (1 - beta2) g'^2
+ *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+ * in 32 bits, t = 1 at the first step; p is rounded to the nearest of its type, so a parameter of 16 bits does not
+ * notice a step below half its spacing.
+ *
+ * The optimizer holds the addresses of the parameters and of their gradients (which the layers keep in place) and the
+ * number of steps; the states belong to the caller, one array each for m and v, in which every tensor begins at a
+ * multiple of 256 elements: fbfc_adamw_state_elements() elements of 4 bytes (state_bits 32) or of one byte (8), 16-byte
+ * aligned, zero at the start.
+ * With 8 bits, 256 consecutive elements share a 32-bit scale (m_scale and v_scale: elements / 256 each, zero at the
+ * start): an element is scale * (its byte as e4m3), scale the largest magnitude of the block over 448, zero for a block
+ * below 2^-100.  Values are rounded up or down at random in proportion to the distance; the random numbers depend on
+ * seed, t and the place alone.  A positive v is held as at least the smallest positive number.  A block that takes an
+ * infinity or a NaN is NaN as a whole from then on.
+ *
+ * Tensors may begin anywhere (aligned to their type) and be empty; a parameter or a state that shares memory with
+ * another tensor is refused.  One step at a time; the step counts itself, so that a step captured into a graph is a
+ * new step at each replay (with the captured lr, weight_decay and grad_scale).  An optimizer works on the device
+ * that was current when it was made. */
+typedef struct {
+    int param_type, grad_type;   /* FBFC_F32, FBFC_BF16 or FBFC_F16 */
+    int state_bits;              /* 32 or 8 */
+    unsigned seed;               /* of the random numbers that 8-bit states are rounded with */
+    double beta1, beta2, eps;    /* in [0, 1), in [0, 1), positive */
+} fbfc_adamw_config;
+typedef struct {
+    void *param;
+    const void *grad;
+    long n;
+} fbfc_adamw_tensor;
+typedef struct fbfc_adamw fbfc_adamw;
+long fbfc_adamw_state_elements(const fbfc_adamw_tensor *tensors, int count);   /* 0 for invalid sizes */
+int fbfc_adamw_create(const fbfc_adamw_config *config, const fbfc_adamw_tensor *tensors, int count, void *m, void *v,
+                      float *m_scale, float *v_scale, fbfc_adamw **opt);
+int fbfc_adamw_destroy(fbfc_adamw *opt);
+int fbfc_adamw_step(fbfc_adamw *opt, double lr, double weight_decay, float grad_scale, void *stream);
+/* The number of steps taken (0 at first), for storing and loading a training state; get waits for the stream. */
+int fbfc_adamw_set_step(fbfc_adamw *opt, long steps, void *stream);
+int fbfc_adamw_get_step(fbfc_adamw *opt, long *steps, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
