@@ -50,6 +50,14 @@ class AdamwTensor(ctypes.Structure):
     _fields_ = [("param", ctypes.c_void_p), ("grad", ctypes.c_void_p), ("n", ctypes.c_long)]
 
 
+class ResidualNormDesc(ctypes.Structure):
+    _fields_ = [("rows", ctypes.c_long), ("channels", ctypes.c_int), ("type", ctypes.c_int), ("eps", ctypes.c_float)]
+
+
+class Rows(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_long)]
+
+
 _vp, _i, _f, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long
 
 # name -> (restype, argtypes); must list every symbol include/fbfftconv.h declares
@@ -94,6 +102,9 @@ SIGNATURES = {
     "fbfc_bias_grad_scratch_bytes": (ctypes.c_size_t, [_i, _i]),
     "fbfc_acc_grad_parameters_bias": (_i, [_vp, _vp, _f, _i, _i, _i, _i, _vp, _vp]),
     "fbfc_acc_grad_parameters_bias_noalloc": (_i, [_vp, _vp, _f, _i, _i, _i, _i, _vp]),
+    "fbfc_residual_norm_forward": (_i, [_vp] * 10),
+    "fbfc_residual_norm_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "fbfc_residual_norm_backward": (_i, [_vp] * 15 + [_f, _vp, _vp]),
     "fbfc_adamw_state_elements": (_l, [ctypes.POINTER(AdamwTensor), _i]),
     "fbfc_adamw_create": (_i, [ctypes.POINTER(AdamwConfig), ctypes.POINTER(AdamwTensor), _i, _vp, _vp, _vp, _vp,
                                ctypes.POINTER(_vp)]),

@@ -55,4 +55,12 @@ __device__ __forceinline__ void store_some(T *p, Vec<T, N> v, long n)
         if (i < n) ((FBFC_GLOBAL T *)p)[i] = v[i];
 }
 
+// sigmoid(z) and sigmoid(-z) = 1 - sigmoid(z), each to its own precision however close the other is to one.
+__device__ __forceinline__ void sigmoid_pair(float z, float &yes, float &no)
+{
+    const float e = __expf(-fabsf(z)), r = 1.0f / (1.0f + e);
+    yes = z < 0.0f ? e * r : r;
+    no = z < 0.0f ? r : e * r;
+}
+
 }  // namespace fbfc

@@ -42,4 +42,28 @@ AdamwClock adamw_clock(long t, double beta1, double beta2, unsigned seed);
 hipError_t launch_adamw(int param_type, int grad_type, int state_bits, const AdamwArgs &a, hipStream_t s);
 hipError_t launch_adamw_set_clock(const AdamwArgs &a, long t, hipStream_t s);
 
+// norm_kernels.hip ------------------------------------------------------------------
+// Rows of one activation tensor: element (r, c) lies r * stride + c values from `data`; absent where data is null.
+struct Rows {
+    void *data;
+    long stride;
+};
+struct NormArgs {
+    long rows;
+    int channels;
+    float eps;
+    Rows residual, branch, gate;
+    const float *post, *scale, *pre;      // with a branch: the first two; with a norm behind it: the last
+    Rows output, normed;                  // forward
+    Rows grad_output, grad_normed;        // backward
+    Rows grad_residual, grad_branch, grad_gate;
+    float *grad_post, *grad_scale, *grad_pre;
+    float factor;                         // of the three gradients above
+    float *partial;                       // norm_workspace_bytes
+};
+constexpr int kNormMaxChannels = 16384;
+size_t norm_workspace_bytes(long rows, int channels, int type);
+hipError_t launch_norm_forward(int type, const NormArgs &a, hipStream_t s);
+hipError_t launch_norm_backward(int type, const NormArgs &a, hipStream_t s);
+
 }  // namespace fbfc

@@ -238,4 +238,137 @@ int fbfc_adamw_step(fbfc_adamw *p, double lr, double weight_decay, float grad_sc
     return FBFC_OK;
 }
 
+// ---- norms around a block --------------------------------------------------------------------------
+static fbfc::Rows rows_of(const fbfc_rows *r)
+{
+    return r == nullptr || r->data == nullptr ? fbfc::Rows{nullptr, 0} : fbfc::Rows{r->data, r->stride};
+}
+
+static int norm_check_desc(const fbfc_residual_norm_desc *d)
+{
+    if (d == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    if (!type_ok(d->type)) return fail(FBFC_ERR_INVALID_ARGUMENT, "unknown type");
+    if (d->rows < 0 || d->channels < 1) return fail(FBFC_ERR_INVALID_ARGUMENT, "sizes must be positive");
+    if (d->channels > fbfc::kNormMaxChannels) {
+        char buf[96];
+        std::snprintf(buf, sizeof buf, "rows of %d channels: up to %d are supported", d->channels, fbfc::kNormMaxChannels);
+        return fail(FBFC_ERR_UNSUPPORTED_SIZE, buf);
+    }
+    if (!(d->eps > 0 && std::isfinite(d->eps))) return fail(FBFC_ERR_INVALID_ARGUMENT, "eps must be positive");
+    return FBFC_OK;
+}
+
+// Alignment, and that the rows of a tensor that is written do not overlap.
+static int norm_check_rows(const fbfc_residual_norm_desc *d, const fbfc::Rows &r, bool written)
+{
+    if (r.data == nullptr) return FBFC_OK;
+    if (!aligned(r.data, type_bytes(d->type))) return fail(FBFC_ERR_INVALID_ARGUMENT, "rows must be aligned to their type");
+    if (r.stride < 0 || (written && d->rows > 1 && r.stride < d->channels))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "rows that are written must not overlap");
+    return FBFC_OK;
+}
+
+static int norm_check_weights(const fbfc::NormArgs &a, bool normed)
+{
+    if (a.gate.data != nullptr && a.branch.data == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "a gate needs a branch");
+    if (a.branch.data != nullptr && (a.post == nullptr || a.scale == nullptr))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "a branch needs its norm's weight and its scale");
+    if (normed && a.pre == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "the norm behind the block needs its weight");
+    return FBFC_OK;
+}
+
+int fbfc_residual_norm_forward(const fbfc_residual_norm_desc *d, const fbfc_rows *residual, const fbfc_rows *branch,
+                               const fbfc_rows *gate, const float *post_weight, const float *scale,
+                               const float *pre_weight, const fbfc_rows *output, const fbfc_rows *normed, void *stream)
+{
+    int rc = norm_check_desc(d);
+    if (rc != FBFC_OK) return rc;
+    fbfc::NormArgs a = {};
+    a.rows = d->rows;
+    a.channels = d->channels;
+    a.eps = d->eps;
+    a.residual = rows_of(residual);
+    a.branch = rows_of(branch);
+    a.gate = rows_of(gate);
+    a.post = post_weight;
+    a.scale = scale;
+    a.pre = pre_weight;
+    a.output = rows_of(output);
+    a.normed = rows_of(normed);
+    if (d->rows == 0) return FBFC_OK;
+    if (a.residual.data == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null residual");
+    if ((a.branch.data == nullptr) != (a.output.data == nullptr))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "the output goes with the branch: without one it is the residual itself");
+    if (a.output.data == nullptr && a.normed.data == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "nothing to compute");
+    rc = norm_check_weights(a, a.normed.data != nullptr);
+    if (rc != FBFC_OK) return rc;
+    for (const fbfc::Rows *r : {&a.residual, &a.branch, &a.gate})
+        if ((rc = norm_check_rows(d, *r, false)) != FBFC_OK) return rc;
+    for (const fbfc::Rows *r : {&a.output, &a.normed})
+        if ((rc = norm_check_rows(d, *r, true)) != FBFC_OK) return rc;
+    fbfc::kernel_log_clear();
+    FBFC_TRY(fbfc::launch_norm_forward(d->type, a, static_cast<hipStream_t>(stream)), "residual norm");
+    return FBFC_OK;
+}
+
+size_t fbfc_residual_norm_workspace_bytes(const fbfc_residual_norm_desc *d)
+{
+    if (d == nullptr || !type_ok(d->type) || d->rows < 1 || d->channels < 1 || d->channels > fbfc::kNormMaxChannels) return 0;
+    return fbfc::norm_workspace_bytes(d->rows, d->channels, d->type);
+}
+
+int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *d, const fbfc_rows *residual, const fbfc_rows *branch,
+                                const fbfc_rows *gate, const float *post_weight, const float *scale,
+                                const float *pre_weight, const fbfc_rows *grad_output, const fbfc_rows *grad_normed,
+                                const fbfc_rows *grad_residual, const fbfc_rows *grad_branch, const fbfc_rows *grad_gate,
+                                float *grad_post_weight, float *grad_scale, float *grad_pre_weight, float factor,
+                                void *workspace, void *stream)
+{
+    int rc = norm_check_desc(d);
+    if (rc != FBFC_OK) return rc;
+    fbfc::NormArgs a = {};
+    a.rows = d->rows;
+    a.channels = d->channels;
+    a.eps = d->eps;
+    a.residual = rows_of(residual);
+    a.branch = rows_of(branch);
+    a.gate = rows_of(gate);
+    a.post = post_weight;
+    a.scale = scale;
+    a.pre = pre_weight;
+    a.grad_output = rows_of(grad_output);
+    a.grad_normed = rows_of(grad_normed);
+    a.grad_residual = rows_of(grad_residual);
+    a.grad_branch = rows_of(grad_branch);
+    a.grad_gate = rows_of(grad_gate);
+    a.grad_post = grad_post_weight;
+    a.grad_scale = grad_scale;
+    a.grad_pre = grad_pre_weight;
+    a.factor = factor;
+    const bool weights = grad_post_weight != nullptr || grad_scale != nullptr || grad_pre_weight != nullptr;
+    if (d->rows > 0) {
+        if (a.residual.data == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null residual");
+        if (a.grad_output.data == nullptr && a.grad_normed.data == nullptr)
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "a gradient of the output or of the norm behind it is needed");
+        if (a.branch.data == nullptr && (a.grad_branch.data != nullptr || grad_post_weight != nullptr || grad_scale != nullptr))
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "there is no branch to have a gradient");
+        if (a.gate.data == nullptr && a.grad_gate.data != nullptr)
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "there is no gate to have a gradient");
+        rc = norm_check_weights(a, a.grad_normed.data != nullptr);
+        if (rc != FBFC_OK) return rc;
+        for (const fbfc::Rows *r : {&a.residual, &a.branch, &a.gate, &a.grad_output, &a.grad_normed})
+            if ((rc = norm_check_rows(d, *r, false)) != FBFC_OK) return rc;
+        for (const fbfc::Rows *r : {&a.grad_residual, &a.grad_branch, &a.grad_gate})
+            if ((rc = norm_check_rows(d, *r, true)) != FBFC_OK) return rc;
+        if (weights && workspace == nullptr)
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "the gradients of the weights need the workspace");
+    } else if ((grad_post_weight != nullptr && scale == nullptr) || (grad_scale != nullptr && post_weight == nullptr)) {
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "a branch needs its norm's weight and its scale");
+    }
+    a.partial = weights ? static_cast<float *>(workspace) : nullptr;
+    fbfc::kernel_log_clear();
+    FBFC_TRY(fbfc::launch_norm_backward(d->type, a, static_cast<hipStream_t>(stream)), "residual norm gradients");
+    return FBFC_OK;
+}
+
 }  // extern "C"

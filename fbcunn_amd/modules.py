@@ -14,11 +14,12 @@ import torch
 
 from . import _lib
 from ._lib import ConvDesc, FbfcError, PlanInfo, check, lib
+from .sequence import GatedResidualNorm
 from .tensors import _check_tensor, _ptr, _stream
 
 __all__ = ["SpatialConvolutionFFT", "SpatialConvolutionFBFFT", "SpatialConvolutionFBFFTGemm", "SpatialConvolutionDirect",
            "SpatialConvolutionFFTTiled", "SpatialConvolutionFFTTiledSync", "SpatialConvolutionFFTTiledAsync",
-           "SpatialConvolutionFFTTiledIterated", "FFTWrapper", "transposeMM", "updateOutputBias", "accGradParametersBias", "FbfcError"]
+           "SpatialConvolutionFFTTiledIterated", "GatedResidualNorm", "FFTWrapper", "transposeMM", "updateOutputBias", "accGradParametersBias", "FbfcError"]
 
 
 class _Plan:

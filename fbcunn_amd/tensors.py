@@ -25,3 +25,19 @@ def _check_tensor(t, name, ndim=None, strided=False):
         raise ValueError("%s must be %d-D" % (name, ndim))
     if not strided and not t.is_contiguous():
         raise ValueError("%s must be contiguous" % name)
+
+
+class Workspace:
+    """Device memory that a module hands to its calls, grown as they need more.  What was outgrown is kept: a graph
+    captured with it may still be replayed."""
+
+    def __init__(self):
+        self._kept = []
+
+    def take(self, nbytes, device):
+        last = self._kept[-1] if self._kept else None
+        if last is None or last.numel() < nbytes or last.device != device:
+            size = max(nbytes, 2 * last.numel() if last is not None and last.device == device else 0, 256)
+            last = torch.empty(size, dtype=torch.uint8, device=device)
+            self._kept.append(last)
+        return last

@@ -386,6 +386,43 @@ int fbfc_adamw_step(fbfc_adamw *opt, double lr, double weight_decay, float grad_
 int fbfc_adamw_set_step(fbfc_adamw *opt, long steps, void *stream);
 int fbfc_adamw_get_step(fbfc_adamw *opt, long *steps, void *stream);
 
+/* The norms before and after a block of a residual network, fused with the block's gate and residual scale.  For each
+ * row of `channels` values, with branch the block's result and rms(x) = sqrt(mean x^2 + eps):
+ *     output = residual + scale * sigmoid(gate) * post_weight * branch / rms(branch)
+ *     normed = pre_weight * output / rms(output)                the next block's input
+ * computed in 32 bits from the inputs and rounded once: normed is the norm of the output before its rounding.  Parts
+ * that are absent (a null pointer, or data null) drop out: without a gate the factor is one; without `normed` there is
+ * no norm behind the block (the last one of a network); without a branch, and so without an output, normed is that of
+ * the residual (before the first block).
+ *
+ * Rows lie `stride` values apart, their channels side by side.  An input's stride may be zero; an output may be an input
+ * of the same address and stride, and overlaps nothing else.  Up to 16384 channels; no rows is no error.
+ *
+ * backward computes the output again from residual, branch and gate, as they went into forward, and takes the gradient
+ * of the output, of normed, or of both.  Every gradient that is not null is assigned; those of the weights, of all rows
+ * times `factor`, are summed in a fixed order through `workspace` (fbfc_residual_norm_workspace_bytes bytes; calls that
+ * may run at the same time need one each). */
+typedef struct {
+    long rows;
+    int channels;
+    int type;      /* of every row: FBFC_F32, FBFC_BF16 or FBFC_F16 */
+    float eps;
+} fbfc_residual_norm_desc;
+typedef struct {
+    void *data;
+    long stride;
+} fbfc_rows;
+int fbfc_residual_norm_forward(const fbfc_residual_norm_desc *desc, const fbfc_rows *residual, const fbfc_rows *branch,
+                               const fbfc_rows *gate, const float *post_weight, const float *scale,
+                               const float *pre_weight, const fbfc_rows *output, const fbfc_rows *normed, void *stream);
+size_t fbfc_residual_norm_workspace_bytes(const fbfc_residual_norm_desc *desc);
+int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_rows *residual, const fbfc_rows *branch,
+                                const fbfc_rows *gate, const float *post_weight, const float *scale,
+                                const float *pre_weight, const fbfc_rows *grad_output, const fbfc_rows *grad_normed,
+                                const fbfc_rows *grad_residual, const fbfc_rows *grad_branch, const fbfc_rows *grad_gate,
+                                float *grad_post_weight, float *grad_scale, float *grad_pre_weight, float factor,
+                                void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
