@@ -58,6 +58,15 @@ class Rows(ctypes.Structure):
     _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_long)]
 
 
+class RecurrenceDesc(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int), ("channels", ctypes.c_int), ("steps", ctypes.c_long), ("type", ctypes.c_int)]
+
+
+class Steps(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("stride_batch", ctypes.c_long), ("stride_step", ctypes.c_long),
+                ("stride_channel", ctypes.c_long)]
+
+
 _vp, _i, _f, _l = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_long
 
 # name -> (restype, argtypes); must list every symbol include/fbfftconv.h declares
@@ -105,6 +114,10 @@ SIGNATURES = {
     "fbfc_residual_norm_forward": (_i, [_vp] * 10),
     "fbfc_residual_norm_workspace_bytes": (ctypes.c_size_t, [_vp]),
     "fbfc_residual_norm_backward": (_i, [_vp] * 15 + [_f, _vp, _vp]),
+    "fbfc_recurrence_checkpoint_bytes": (ctypes.c_size_t, [_vp]),
+    "fbfc_recurrence_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "fbfc_recurrence_forward": (_i, [_vp] * 11),
+    "fbfc_recurrence_backward": (_i, [_vp] * 11 + [_f] + [_vp] * 3),
     "fbfc_adamw_state_elements": (_l, [ctypes.POINTER(AdamwTensor), _i]),
     "fbfc_adamw_create": (_i, [ctypes.POINTER(AdamwConfig), ctypes.POINTER(AdamwTensor), _i, _vp, _vp, _vp, _vp,
                                ctypes.POINTER(_vp)]),

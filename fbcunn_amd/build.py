@@ -19,7 +19,7 @@ PROBE_LIB = os.path.join(HERE, "libfbfftconv_probe.so")
 PROBE_SOURCES = [("cgemm_kernels.hip", "cgemm_kernels_probe.o", ["-DFBFC_PROBES"]),
                  ("probe_clock.cpp", "probe_clock.o", ["-DFBFC_PROBES"])]
 SOURCES = ["api.cpp", "fft_kernels.hip", "fft_large.hip", "fft_small.hip", "cgemm_kernels.hip", "bias_kernels.hip", "bias_noalloc.hip", "layout_kernels.hip", "direct_kernels.hip", "fused_kernels.hip",
-           "training_api.cpp", "adamw_kernels.hip", "norm_kernels.hip"]
+           "training_api.cpp", "adamw_kernels.hip", "norm_kernels.hip", "recurrence_kernels.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [
     "--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-x", "hip",

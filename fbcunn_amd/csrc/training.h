@@ -66,4 +66,30 @@ size_t norm_workspace_bytes(long rows, int channels, int type);
 hipError_t launch_norm_forward(int type, const NormArgs &a, hipStream_t s);
 hipError_t launch_norm_backward(int type, const NormArgs &a, hipStream_t s);
 
+// recurrence_kernels.hip -------------------------------------------------------------
+// One activation tensor over (batch, step, channel), strides in values; absent where data is null.
+struct Steps {
+    void *data;
+    long sb, st, sc;
+};
+struct RecArgs {
+    int batch, channels;
+    long steps;
+    Steps x, gate, y;              // y: the output, or the gradient of the output
+    Steps grad_x, grad_gate;
+    const float *bias;
+    const int *lengths;
+    const float *state_in;         // backward: the gradient of the state behind the last step
+    float *state_out;              // backward: the gradient of the state before the first step
+    float *checkpoints;            // the state before each tile of steps: (tiles, batch, channels)
+    float *grad_bias;
+    float factor;                  // of grad_bias
+    unsigned char *workspace;
+};
+size_t recurrence_checkpoint_bytes(int batch, int channels, long steps);
+size_t recurrence_workspace_bytes(int batch, int channels, long steps);
+bool recurrence_fits(int batch, int channels, long steps);
+hipError_t launch_recurrence_forward(int type, const RecArgs &a, hipStream_t s);
+hipError_t launch_recurrence_backward(int type, const RecArgs &a, hipStream_t s);
+
 }  // namespace fbfc

@@ -371,4 +371,125 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *d, const fbfc_row
     return FBFC_OK;
 }
 
+// ---- gated linear recurrence -----------------------------------------------------------------------
+static fbfc::Steps steps_of(const fbfc_steps *t)
+{
+    return t == nullptr || t->data == nullptr ? fbfc::Steps{nullptr, 0, 0, 0}
+                                              : fbfc::Steps{t->data, t->stride_batch, t->stride_step, t->stride_channel};
+}
+
+static int recurrence_check_desc(const fbfc_recurrence_desc *d)
+{
+    if (d == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    if (!type_ok(d->type)) return fail(FBFC_ERR_INVALID_ARGUMENT, "unknown type");
+    if (d->batch < 0 || d->steps < 0 || d->channels < 1) return fail(FBFC_ERR_INVALID_ARGUMENT, "sizes must be positive");
+    if (d->batch > 0 && (d->steps > (1L << 40) || !fbfc::recurrence_fits(d->batch, d->channels, d->steps)))
+        return fail(FBFC_ERR_UNSUPPORTED_SIZE, "more sequences, channels and steps than one launch can take");
+    return FBFC_OK;
+}
+
+static int recurrence_check_steps(const fbfc_recurrence_desc *d, const fbfc::Steps &t, bool written)
+{
+    if (t.data == nullptr) return FBFC_OK;
+    if (!aligned(t.data, type_bytes(d->type))) return fail(FBFC_ERR_INVALID_ARGUMENT, "tensors must be aligned to their type");
+    if (!written) return FBFC_OK;
+    // the places of a tensor that is written must differ: with its dimensions ordered by stride, each stride passes
+    // over all that the smaller ones reach
+    struct Dim {
+        long n, stride;
+    } dims[3] = {{d->batch, t.sb}, {d->steps, t.st}, {d->channels, t.sc}};
+    std::sort(dims, dims + 3, [](const Dim &x, const Dim &y) { return x.stride < y.stride; });
+    long reach = 0;  // of the smaller strides
+    for (const Dim &x : dims) {
+        if (x.n < 2) continue;
+        if (x.stride <= reach || x.stride > (1L << 60) / x.n)
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "strides of a tensor that is written must not overlap or be negative");
+        reach += x.stride * (x.n - 1);
+    }
+    return FBFC_OK;
+}
+
+size_t fbfc_recurrence_checkpoint_bytes(const fbfc_recurrence_desc *d)
+{
+    if (d == nullptr || d->batch < 1 || d->steps < 1 || d->channels < 1) return 0;
+    return fbfc::recurrence_checkpoint_bytes(d->batch, d->channels, d->steps);
+}
+
+size_t fbfc_recurrence_workspace_bytes(const fbfc_recurrence_desc *d)
+{
+    if (d == nullptr || d->batch < 1 || d->steps < 1 || d->channels < 1) return 0;
+    return fbfc::recurrence_workspace_bytes(d->batch, d->channels, d->steps);
+}
+
+int fbfc_recurrence_forward(const fbfc_recurrence_desc *d, const fbfc_steps *input, const fbfc_steps *gate,
+                            const float *gate_bias, const float *state_in, const int *lengths, const fbfc_steps *output,
+                            float *state_out, float *checkpoints, void *workspace, void *stream)
+{
+    int rc = recurrence_check_desc(d);
+    if (rc != FBFC_OK) return rc;
+    fbfc::RecArgs a = {};
+    a.batch = d->batch;
+    a.channels = d->channels;
+    a.steps = d->steps;
+    a.x = steps_of(input);
+    a.gate = steps_of(gate);
+    a.y = steps_of(output);
+    a.bias = gate_bias;
+    a.state_in = state_in;
+    a.lengths = lengths;
+    a.state_out = state_out;
+    a.checkpoints = checkpoints;
+    a.workspace = static_cast<unsigned char *>(workspace);
+    if (d->batch == 0) return FBFC_OK;
+    if (d->steps > 0) {
+        if (a.x.data == nullptr || a.gate.data == nullptr || a.y.data == nullptr)
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "input, gate and output are needed");
+        for (const fbfc::Steps *t : {&a.x, &a.gate, &a.y})
+            if ((rc = recurrence_check_steps(d, *t, t == &a.y)) != FBFC_OK) return rc;
+        if (d->steps > 1 && (workspace == nullptr || !aligned(workspace, 16)))
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "a workspace aligned to 16 bytes is needed");
+    }
+    fbfc::kernel_log_clear();
+    FBFC_TRY(fbfc::launch_recurrence_forward(d->type, a, static_cast<hipStream_t>(stream)), "recurrence");
+    return FBFC_OK;
+}
+
+int fbfc_recurrence_backward(const fbfc_recurrence_desc *d, const fbfc_steps *input, const fbfc_steps *gate,
+                             const float *gate_bias, const int *lengths, const float *checkpoints,
+                             const fbfc_steps *grad_output, const float *grad_state_out, const fbfc_steps *grad_input,
+                             const fbfc_steps *grad_gate, float *grad_gate_bias, float factor, float *grad_state_in,
+                             void *workspace, void *stream)
+{
+    int rc = recurrence_check_desc(d);
+    if (rc != FBFC_OK) return rc;
+    fbfc::RecArgs a = {};
+    a.batch = d->batch;
+    a.channels = d->channels;
+    a.steps = d->steps;
+    a.x = steps_of(input);
+    a.gate = steps_of(gate);
+    a.y = steps_of(grad_output);
+    a.grad_x = steps_of(grad_input);
+    a.grad_gate = steps_of(grad_gate);
+    a.bias = gate_bias;
+    a.state_in = grad_state_out;
+    a.lengths = lengths;
+    a.state_out = grad_state_in;
+    a.checkpoints = const_cast<float *>(checkpoints);
+    a.grad_bias = grad_gate_bias;
+    a.factor = factor;
+    a.workspace = static_cast<unsigned char *>(workspace);
+    if (d->batch > 0 && d->steps > 0) {
+        if (a.x.data == nullptr || a.gate.data == nullptr || a.y.data == nullptr || checkpoints == nullptr)
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "input, gate, the output's gradient and the checkpoints are needed");
+        for (const fbfc::Steps *t : {&a.x, &a.gate, &a.y, &a.grad_x, &a.grad_gate})
+            if ((rc = recurrence_check_steps(d, *t, t == &a.grad_x || t == &a.grad_gate)) != FBFC_OK) return rc;
+        if (workspace == nullptr || !aligned(workspace, 16))
+            return fail(FBFC_ERR_INVALID_ARGUMENT, "a workspace aligned to 16 bytes is needed");
+    }
+    fbfc::kernel_log_clear();
+    FBFC_TRY(fbfc::launch_recurrence_backward(d->type, a, static_cast<hipStream_t>(stream)), "recurrence gradients");
+    return FBFC_OK;
+}
+
 }  // extern "C"

@@ -14,12 +14,13 @@ import torch
 
 from . import _lib
 from ._lib import ConvDesc, FbfcError, PlanInfo, check, lib
-from .sequence import GatedResidualNorm
+from .sequence import GatedLinearRecurrence, GatedResidualNorm
 from .tensors import _check_tensor, _ptr, _stream
 
 __all__ = ["SpatialConvolutionFFT", "SpatialConvolutionFBFFT", "SpatialConvolutionFBFFTGemm", "SpatialConvolutionDirect",
            "SpatialConvolutionFFTTiled", "SpatialConvolutionFFTTiledSync", "SpatialConvolutionFFTTiledAsync",
-           "SpatialConvolutionFFTTiledIterated", "GatedResidualNorm", "FFTWrapper", "transposeMM", "updateOutputBias", "accGradParametersBias", "FbfcError"]
+           "SpatialConvolutionFFTTiledIterated", "GatedLinearRecurrence",
+           "GatedResidualNorm", "FFTWrapper", "transposeMM", "updateOutputBias", "accGradParametersBias", "FbfcError"]
 
 
 class _Plan:

@@ -5,10 +5,10 @@ import ctypes
 import torch
 
 from . import _lib
-from ._lib import ResidualNormDesc, Rows, check, lib
+from ._lib import RecurrenceDesc, ResidualNormDesc, Rows, Steps, check, lib
 from .tensors import TYPES, Workspace, _ptr, _stream
 
-__all__ = ["GatedResidualNorm"]
+__all__ = ["GatedLinearRecurrence", "GatedResidualNorm"]
 
 
 def _check_activation(t, name, like=None):
@@ -23,6 +23,156 @@ def _check_activation(t, name, like=None):
             raise TypeError("%s must be %s" % (name, like.dtype))
         if t.shape != like.shape:
             raise ValueError("%s has the wrong shape" % name)
+
+
+def _like(old, t):
+    """`old` where it can take what has the shape and the type of t, else a new tensor."""
+    if old is not None and old.shape == t.shape and old.dtype == t.dtype and old.device == t.device:
+        return old
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+
+
+def _steps(t):
+    return None if t is None else ctypes.byref(Steps(t.data_ptr(), *t.stride()))
+
+
+class GatedLinearRecurrence:
+    """a_t = sigmoid(gate_t + bias), state = a_t state + (1 - a_t) x_t, output_t = state, for every sequence and channel.
+
+    updateOutput takes [x, gate], both (batch, steps, nChannels), float32, bfloat16 or float16, of any strides, and gives the
+    output, of the same shape; self.state is then the state behind the last step (batch, nChannels) in float32.
+    `state`: the state before the first step, zeros where it is None.  `lengths`: an int32 CUDA tensor with the steps of each
+    sequence; behind them nothing is read, and outputs and gradients are zero.  backward (and its halves updateGradInput
+    and accGradParameters) follows an updateOutput of the same inputs, from which the module keeps the state before every
+    128 steps; after evaluate() it keeps none and cannot go backward.  step advances sequences by one token."""
+
+    def __init__(self, nChannels, device="cuda"):
+        if not isinstance(nChannels, int) or nChannels < 1:
+            raise ValueError("nChannels must be a positive number")
+        self.nChannels = nChannels
+        self.device = torch.device(device)
+        self.bias = torch.zeros(nChannels, device=self.device)
+        self.gradBias = torch.zeros(nChannels, device=self.device)
+        self.train = True
+        self.output = self.state = self.gradInput = self.gradState = None
+        self._workspace, self._checkpoints = Workspace(), Workspace()
+        self._forward = None   # (shape, type, lengths, checkpoints) of the updateOutput that backward may follow
+
+    def training(self):
+        self.train = True
+
+    def evaluate(self):
+        self.train = False
+
+    def parameters(self):
+        return [self.bias], [self.gradBias]
+
+    def zeroGradParameters(self):
+        self.gradBias.zero_()
+
+    def _inputs(self, input):
+        if len(input) != 2:
+            raise ValueError("the input is [x, gate]")
+        x, gate = input
+        _check_activation(x, "x")
+        _check_activation(gate, "gate", x)
+        if x.dim() != 3 or x.size(2) != self.nChannels:
+            raise ValueError("x must be (batch, steps, %d)" % self.nChannels)
+        return x, gate, ctypes.byref(RecurrenceDesc(x.size(0), self.nChannels, x.size(1), TYPES[x.dtype]))
+
+    def _check_state(self, t, name, batch):
+        if t is None:
+            return
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TypeError("%s: CUDA support only!" % name)
+        if t.dtype != torch.float32:
+            raise TypeError("%s must be float32" % name)
+        if tuple(t.shape) != (batch, self.nChannels) or not t.is_contiguous() or t.device.index != torch.cuda.current_device():
+            raise ValueError("%s must be a contiguous (%d, %d) tensor on the current device" % (name, batch, self.nChannels))
+
+    @staticmethod
+    def _check_lengths(t, batch):
+        if t is None:
+            return
+        if not isinstance(t, torch.Tensor) or not t.is_cuda:
+            raise TypeError("lengths: CUDA support only!")
+        if t.dtype != torch.int32:
+            raise TypeError("lengths must be int32")
+        if tuple(t.shape) != (batch,) or not t.is_contiguous() or t.device.index != torch.cuda.current_device():
+            raise ValueError("lengths must be %d contiguous numbers on the current device" % batch)
+
+    def updateOutput(self, input, state=None, lengths=None):
+        x, gate, desc = self._inputs(input)
+        batch = x.size(0)
+        self._check_state(state, "state", batch)
+        self._check_lengths(lengths, batch)
+        self.output = _like(self.output, x)
+        if self.state is None or self.state.size(0) != batch or self.state.device != x.device:
+            self.state = torch.empty(batch, self.nChannels, device=x.device)
+        kept = None
+        if self.train:
+            kept = self._checkpoints.take(lib().fbfc_recurrence_checkpoint_bytes(desc), x.device)
+        ws = self._workspace.take(lib().fbfc_recurrence_workspace_bytes(desc), x.device)
+        self._forward = None
+        check(lib().fbfc_recurrence_forward(desc, _steps(x), _steps(gate), _ptr(self.bias), _ptr(state), _ptr(lengths),
+                                            _steps(self.output), _ptr(self.state), _ptr(kept), _ptr(ws), _stream()))
+        if self.train:
+            self._forward = (x.shape, x.dtype, lengths, kept)
+        return self.output
+
+    forward = updateOutput
+
+    def step(self, input, state):
+        """One token of each sequence: [x, gate] of (batch, nChannels); advances `state` in place and gives the output."""
+        if len(input) != 2:
+            raise ValueError("the input is [x, gate]")
+        x, gate = input
+        _check_activation(x, "x")
+        _check_activation(gate, "gate", x)
+        if x.dim() != 2 or x.size(1) != self.nChannels:
+            raise ValueError("x must be (batch, %d)" % self.nChannels)
+        if state is None:
+            raise TypeError("step needs the state that it advances")
+        self._check_state(state, "state", x.size(0))
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+        tensors = [ctypes.byref(Steps(t.data_ptr(), t.stride(0), 0, t.stride(1))) for t in (x, gate, out)]
+        desc = RecurrenceDesc(x.size(0), self.nChannels, 1, TYPES[x.dtype])
+        check(lib().fbfc_recurrence_forward(ctypes.byref(desc), tensors[0], tensors[1], _ptr(self.bias), _ptr(state), None,
+                                            tensors[2], _ptr(state), None, None, _stream()))
+        return out
+
+    def _backward(self, input, gradOutput, gradState, inputs, weights, scale):
+        x, gate, desc = self._inputs(input)
+        if self._forward is None or self._forward[:2] != (x.shape, x.dtype):
+            raise ValueError("backward follows an updateOutput of the same inputs, not after evaluate()")
+        _check_activation(gradOutput, "gradOutput", x)
+        self._check_state(gradState, "gradState", x.size(0))
+        grads, first = [None, None], None
+        if inputs:
+            old = self.gradInput or [None, None]
+            self.gradInput = [_like(old[0], x), _like(old[1], x)]
+            grads = [_steps(t) for t in self.gradInput]
+            if self.gradState is None or self.gradState.size(0) != x.size(0) or self.gradState.device != x.device:
+                self.gradState = torch.empty(x.size(0), self.nChannels, device=x.device)
+            first = self.gradState
+        ws = self._workspace.take(lib().fbfc_recurrence_workspace_bytes(desc), x.device)
+        check(lib().fbfc_recurrence_backward(desc, _steps(x), _steps(gate), _ptr(self.bias), _ptr(self._forward[2]),
+                                             _ptr(self._forward[3]), _steps(gradOutput), _ptr(gradState), *grads,
+                                             _ptr(self.gradBias if weights else None), scale, _ptr(first), _ptr(ws), _stream()))
+
+    def updateGradInput(self, input, gradOutput, gradState=None):
+        """[gradient of x, gradient of gate]; self.gradState is the gradient of the state before the first step.  `gradState`:
+        the gradient of the state behind the last one."""
+        self._backward(input, gradOutput, gradState, True, False, 1.0)
+        return self.gradInput
+
+    def accGradParameters(self, input, gradOutput, scale=1.0, gradState=None):
+        self._backward(input, gradOutput, gradState, False, True, scale)
+
+    def backward(self, input, gradOutput, scale=1.0, gradState=None):
+        """updateGradInput and accGradParameters in one pass over the inputs."""
+        self._backward(input, gradOutput, gradState, True, True, scale)
+        return self.gradInput
 
 
 class GatedResidualNorm:
@@ -87,19 +237,12 @@ class GatedResidualNorm:
         desc = ResidualNormDesc(residual.numel() // self.nChannels, self.nChannels, TYPES[residual.dtype], self.eps)
         return ctypes.byref(desc), residual, [self._rows(t, n) for t, n in zip(input, names)] + [None] * (3 - len(names))
 
-    @staticmethod
-    def _like(old, t):
-        """`old` where it can take what has the shape and the type of t, else a new tensor."""
-        if old is not None and old.shape == t.shape and old.dtype == t.dtype and old.device == t.device:
-            return old
-        return torch.empty(t.shape, dtype=t.dtype, device=t.device)
-
     def updateOutput(self, input):
         desc, residual, rows = self._inputs(input)
         old = self.output or [None, None]
         # without a branch the first output is the caller's tensor, never one to write into
-        output = self._like(old[0], residual) if self.hasBranch else None
-        normed = self._like(old[1], residual) if self.hasNorm else None
+        output = _like(old[0], residual) if self.hasBranch else None
+        normed = _like(old[1], residual) if self.hasNorm else None
         check(lib().fbfc_residual_norm_forward(desc, *rows, _ptr(self.postWeight), _ptr(self.scale), _ptr(self.preWeight),
                                                self._rows(output, "output"), self._rows(normed, "normed"), _stream()))
         self.output = [output if self.hasBranch else residual, normed]
@@ -121,7 +264,7 @@ class GatedResidualNorm:
         if inputs:
             old = self.gradInput or [None] * 3
             n = 1 + self.hasBranch + self.hasGate
-            self.gradInput = [self._like(old[i], residual) for i in range(n)]
+            self.gradInput = [_like(old[i], residual) for i in range(n)]
             grads = [self._rows(t, "gradInput") for t in self.gradInput] + [None] * (3 - n)
         ws, params = None, [None] * 3
         if weights:

@@ -423,6 +423,45 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_
                                 float *grad_post_weight, float *grad_scale, float *grad_pre_weight, float factor,
                                 void *workspace, void *stream);
 
+/* The gated linear recurrence: for each sequence b and channel c, from the state before the first step on,
+ *     a_t = sigmoid(gate_t + gate_bias)      state = a_t state + (1 - a_t) input_t      output_t = state
+ * with the state in 32 bits throughout and each output rounded once.
+ *
+ * Element (b, t, c) of a tensor lies b * stride_batch + t * stride_step + c * stride_channel values from `data`, any
+ * strides for what is read; channels side by side (stride_channel 1) are the fast order, steps side by side, as in the
+ * planes of a convolution, are supported.  gate_bias has `channels` values, the states (batch, channels); null stands
+ * for zeros.  state_out may be null, or be state_in.  The output may be one of the inputs with the same strides.
+ * `lengths` (null: all of full length) holds the number of steps of each sequence, on the device, taken as between 0
+ * and `steps`: what lies behind them is not read, and the output and the gradients there are zero; state_out is the
+ * state behind the last of them.  No steps or no sequences is no error: the state passes through.  One step is the form
+ * for serving: one launch, and no workspace.
+ *
+ * `checkpoints` (fbfc_recurrence_checkpoint_bytes bytes, null where no gradient follows) keeps the state before each
+ * 128 steps for backward, which takes the same descriptor, inputs and lengths.  backward assigns each gradient that is
+ * not null; that of gate_bias is the sum over sequences and steps, in a fixed order, times `factor`.  grad_state_out,
+ * the gradient of state_out, may be null, or be grad_state_in.
+ * `workspace`: fbfc_recurrence_workspace_bytes bytes, 16-byte aligned, of any content; calls that may run at the same
+ * time need one each. */
+typedef struct {
+    int batch, channels;
+    long steps;
+    int type;      /* of input, gate, output and their gradients: FBFC_F32, FBFC_BF16 or FBFC_F16 */
+} fbfc_recurrence_desc;
+typedef struct {
+    void *data;
+    long stride_batch, stride_step, stride_channel;
+} fbfc_steps;
+size_t fbfc_recurrence_checkpoint_bytes(const fbfc_recurrence_desc *desc);
+size_t fbfc_recurrence_workspace_bytes(const fbfc_recurrence_desc *desc);
+int fbfc_recurrence_forward(const fbfc_recurrence_desc *desc, const fbfc_steps *input, const fbfc_steps *gate,
+                            const float *gate_bias, const float *state_in, const int *lengths, const fbfc_steps *output,
+                            float *state_out, float *checkpoints, void *workspace, void *stream);
+int fbfc_recurrence_backward(const fbfc_recurrence_desc *desc, const fbfc_steps *input, const fbfc_steps *gate,
+                             const float *gate_bias, const int *lengths, const float *checkpoints,
+                             const fbfc_steps *grad_output, const float *grad_state_out, const fbfc_steps *grad_input,
+                             const fbfc_steps *grad_gate, float *grad_gate_bias, float factor, float *grad_state_in,
+                             void *workspace, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

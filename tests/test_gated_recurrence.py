@@ -1,0 +1,441 @@
+"""The gated linear recurrence (nn.GatedLinearRecurrence, fbfc_recurrence_*): values and gradients against one step after
+the other in 64 bits, with bounds that are carried through the same recurrence."""
+import ctypes
+
+import pytest
+import torch
+
+from fbcunn_amd import _lib
+
+U = 2.0 ** -24
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+
+
+# refusals: no GPU needed ------------------------------------------------------------------------------
+
+P = 0x1000
+
+
+def _st(data=P, sb=80, st=8, sc=1):
+    return ctypes.byref(_lib.Steps(data, sb, st, sc))
+
+
+def _forward(batch=2, channels=8, steps=10, type=0, **kw):
+    d = _lib.RecurrenceDesc(batch, channels, steps, type)
+    a = dict(x=_st(), gate=_st(), bias=None, state_in=None, lengths=None, y=_st(), state_out=P, checkpoints=None, workspace=P)
+    a.update(kw)
+    rc = _lib.lib().fbfc_recurrence_forward(ctypes.byref(d), *a.values(), None)
+    return rc, _lib.lib().fbfc_last_error().decode()
+
+
+def _backward(batch=2, channels=8, steps=10, type=0, **kw):
+    d = _lib.RecurrenceDesc(batch, channels, steps, type)
+    a = dict(x=_st(), gate=_st(), bias=None, lengths=None, checkpoints=P, y=_st(), gstate=None, gx=_st(), gz=_st(), gb=P, factor=1.0,
+             gstate_in=P, workspace=P)
+    a.update(kw)
+    rc = _lib.lib().fbfc_recurrence_backward(ctypes.byref(d), *a.values(), None)
+    return rc, _lib.lib().fbfc_last_error().decode()
+
+
+@pytest.mark.parametrize("call", [_forward, _backward])
+@pytest.mark.parametrize("kw,text", [
+    (dict(batch=-1), "positive"), (dict(channels=0), "positive"), (dict(steps=-1), "positive"), (dict(type=7), "type"),
+    (dict(x=None), "needed"), (dict(gate=_st(0)), "needed"), (dict(y=None), "needed"), (dict(x=_st(0x1002)), "aligned"),
+    (dict(workspace=None), "workspace"), (dict(workspace=0x1008), "workspace"),
+])
+def test_refusals(call, kw, text):
+    rc, message = call(**kw)
+    assert rc == _lib.ERR_INVALID_ARGUMENT and text in message, message
+
+
+def test_more_refusals():
+    for bad in (_st(sb=79), _st(st=7), _st(sc=0), _st(sb=-80), _st(sb=8, st=8), _st(sb=80, st=1, sc=9)):
+        rc, message = _forward(y=bad)
+        assert rc == _lib.ERR_INVALID_ARGUMENT and "overlap" in message
+        for k in ("gx", "gz"):
+            rc, message = _backward(**{k: bad})
+            assert rc == _lib.ERR_INVALID_ARGUMENT and "overlap" in message
+    rc, message = _backward(checkpoints=None)
+    assert rc == _lib.ERR_INVALID_ARGUMENT and "checkpoints" in message
+    assert _forward(batch=1 << 30, channels=1 << 30)[0] == _lib.ERR_UNSUPPORTED_SIZE
+    assert _forward(batch=1 << 20, channels=1 << 17, steps=1 << 39)[0] == _lib.ERR_UNSUPPORTED_SIZE
+    L = _lib.lib()
+    assert L.fbfc_recurrence_forward(None, *([None] * 10)) == _lib.ERR_INVALID_ARGUMENT
+    assert L.fbfc_recurrence_checkpoint_bytes(None) == 0 and L.fbfc_recurrence_workspace_bytes(None) == 0
+    assert _forward(batch=0)[0] == _lib.OK
+
+
+def test_checkpoints_are_small():
+    d = _lib.RecurrenceDesc(3, 100, 1000, _lib.BF16)
+    assert _lib.lib().fbfc_recurrence_checkpoint_bytes(ctypes.byref(d)) == 3 * 100 * 8 * 4
+
+
+def test_module_refusals_without_gpu():
+    from fbcunn_amd import nn
+    with pytest.raises(ValueError):
+        nn.GatedLinearRecurrence(0, device="cpu")
+    with pytest.raises(TypeError):
+        nn.GatedLinearRecurrence(8, device="cpu").updateOutput([torch.zeros(2, 3, 8)] * 2)
+
+
+# plain form ----------------------------------------------------------------------------------------------
+
+def _plain(x, gate, bias, h0=None, lengths=None, gy=None, gh=None, factor=1.0):
+    """{name: (value, bound before the last rounding)}, one step after the other in 64 bits.  The bounds count, for gates
+    below 10: 24 units of 1 - a (its exponential is off by |z| + 2), 10 of a, 2 of each sum."""
+    up = lambda t: None if t is None else t.detach().cpu().double()   # noqa: E731
+    x, gate, bias, gy, gh = up(x), up(gate), up(bias), up(gy), up(gh)
+    B, T, D = x.shape
+    n = torch.full((B,), T) if lengths is None else lengths.cpu().clamp(0, T)
+    z = gate + bias
+    a, c = torch.sigmoid(z), torch.sigmoid(-z)
+    live = torch.arange(T)[None, :, None] < n[:, None, None]
+    x, a, c = torch.where(live, x, 0.0), torch.where(live, a, 1.0), torch.where(live, c, 0.0)
+    h = torch.zeros(B, D, dtype=torch.float64) if h0 is None else up(h0).clone()
+    e = torch.zeros_like(h)
+    H, E, before, Eb = (torch.zeros(B, T, D, dtype=torch.float64) for _ in range(4))
+    for t in range(T):
+        before[:, t], Eb[:, t] = h, e
+        new = a[:, t] * h + c[:, t] * x[:, t]
+        e = a[:, t] * e + U * (24 * c[:, t] * (x[:, t].abs() + h.abs()) + 10 * a[:, t] * h.abs() + 2 * new.abs())
+        h = new
+        H[:, t], E[:, t] = h, e
+    res = {"output": (torch.where(live, H, 0.0), torch.where(live, E, 0.0)), "state": (h, e)}
+    if gy is None:
+        return res
+    gy = torch.where(live, gy, 0.0)
+    g = torch.zeros(B, D, dtype=torch.float64) if gh is None else gh.clone()
+    f = torch.zeros_like(g)
+    u, F = torch.zeros_like(H), torch.zeros_like(H)
+    for t in range(T - 1, -1, -1):
+        u[:, t] = gy[:, t] + g
+        F[:, t] = f + 2 * U * u[:, t].abs()
+        # magnitudes: a sum that cancels was still rounded at the size of its parts
+        size = gy[:, t].abs() + g.abs()
+        g = a[:, t] * u[:, t]
+        f = a[:, t] * (F[:, t] + 14 * U * size)
+    d = before - x
+    gz = u * d * a * c
+    err = a * c * (F * d.abs() + u.abs() * (Eb + U * (before.abs() + x.abs())) + 48 * U * u.abs() * d.abs())
+    res["gradX"] = (c * u, c * F + 26 * U * (c * u).abs())
+    res["gradGate"] = (gz, err)
+    res["gradState"] = (g, f)
+    adds = 40 + B * (T // 16 + 1) / 16
+    res["gradBias"] = (gz.sum((0, 1)) * factor, abs(factor) * (err.sum((0, 1)) + adds * U * gz.abs().sum((0, 1))))
+    return res
+
+
+def _check(got, want, what):
+    value, bound = want
+    x = got.detach().cpu().double()
+    tol = bound + U * value.abs() + 1e-37
+    if got.dtype != torch.float32:
+        tol = bound + torch.finfo(got.dtype).eps / 2 * (value.abs() + bound) + (2.0 ** -25 if got.dtype == torch.float16 else 1e-37)
+    off = (x - value).abs()
+    assert bool((off <= tol).all()), "%s: %g times the bound" % (what, float((off / tol).max()))
+
+
+def _data(B, T, D, dtype, seed, order="btd"):
+    gen = torch.Generator("cuda").manual_seed(seed)
+    if order == "bdt":    # steps side by side, as in the planes of a convolution
+        make = lambda s=1.0: (torch.randn(B, D, T, generator=gen, device="cuda") * s).to(dtype).transpose(1, 2)   # noqa: E731
+    elif order == "tbd":
+        make = lambda s=1.0: (torch.randn(T, B, D, generator=gen, device="cuda") * s).to(dtype).transpose(0, 1)   # noqa: E731
+    else:
+        make = lambda s=1.0: (torch.randn(B, T, D, generator=gen, device="cuda") * s).to(dtype)   # noqa: E731
+    from fbcunn_amd import nn
+    net = nn.GatedLinearRecurrence(D)
+    net.bias.copy_(torch.rand(D, generator=gen, device="cuda") * 6 - 1)
+    h0, gh = (torch.randn(B, D, generator=gen, device="cuda") for _ in range(2))
+    return net, make(), make(), make(), h0, gh
+
+
+def _check_all(net, x, gate, gy, h0, gh, lengths=None, factor=1.0):
+    want = _plain(x, gate, net.bias, h0, lengths, gy, gh, factor)
+    y = net.updateOutput([x, gate], state=h0, lengths=lengths)
+    net.backward([x, gate], gy, factor, gradState=gh)
+    for name, got in (("output", y), ("state", net.state), ("gradX", net.gradInput[0]), ("gradGate", net.gradInput[1]),
+                      ("gradState", net.gradState), ("gradBias", net.gradBias)):
+        _check(got, want[name], name)
+
+
+SHAPES = [(1, 1, 1), (3, 1, 130), (2, 2, 3), (5, 15, 64), (2, 16, 63), (1, 17, 2), (3, 100, 129), (2, 127, 65), (1, 128, 257),
+          (4, 129, 515), (2, 255, 1), (1, 256, 128), (3, 300, 33), (1, 1000, 130), (2, 2500, 50), (1, 5000, 7)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "%dx%dx%d" % s)
+def test_values_and_gradients(shape, dtype):
+    _check_all(*_data(*shape, TYPES[dtype], sum(shape)), factor=0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("shape", [(260, 300, 130), (1030, 130, 5)], ids=lambda s: "%dx%dx%d" % s)
+def test_one_workgroup_walks_over_the_tiles(shape, dtype):
+    data = _data(*shape, TYPES[dtype], 3)
+    _check_all(*data)
+    assert "chain" not in _lib.lib().fbfc_last_launch().decode()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("order", ["bdt", "tbd"])
+@pytest.mark.parametrize("shape", [(3, 1, 20), (3, 40, 20), (2, 300, 70)], ids=lambda s: "%dx%dx%d" % s)
+def test_other_orders(shape, order):
+    _check_all(*_data(*shape, torch.float32, 5, order))
+
+
+@pytest.mark.gpu
+def test_broadcast_gate_and_no_state():
+    net, x, gate, gy, _, _ = _data(3, 200, 70, torch.bfloat16, 6)
+    want = _plain(x, gate[:1, :1].expand_as(x), net.bias, None, None, gy, None)
+    wide = gate[:1, :1].expand_as(x)
+    _check(net.updateOutput([x, wide]), want["output"], "output")
+    net.backward([x, wide], gy)
+    _check(net.gradInput[1], want["gradGate"], "gradGate")
+    _check(net.gradState, want["gradState"], "gradState")
+    net.bias.zero_()
+    want = _plain(x, gate, net.bias)
+    _check(net.updateOutput([x, gate]), want["output"], "output")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 20, 300, 1300])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_padded_batch(T, dtype):
+    """Lengths of zero, one, all, and out of range; what lies behind them is no number and is not read."""
+    net, x, gate, gy, h0, gh = _data(6, T, 131, TYPES[dtype], 7)
+    lengths = torch.tensor([0, 1, T, T - T // 3, T + 5, -2], dtype=torch.int32, device="cuda")
+    for b, n in enumerate(lengths.clamp(0, T).tolist()):
+        for t, v in ((x, float("nan")), (gate, float("inf")), (gy, float("nan"))):
+            t[b, n:] = v
+    clean = [torch.nan_to_num(t.float(), 0.0, 0.0, 0.0) for t in (x, gate, gy)]
+    want = _plain(clean[0], clean[1], net.bias, h0, lengths, clean[2], gh)
+    y = net.updateOutput([x, gate], state=h0, lengths=lengths)
+    net.output.fill_(float("nan"))
+    y = net.updateOutput([x, gate], state=h0, lengths=lengths)
+    net.backward([x, gate], gy, gradState=gh)
+    for name, got in (("output", y), ("state", net.state), ("gradX", net.gradInput[0]), ("gradGate", net.gradInput[1]),
+                      ("gradState", net.gradState), ("gradBias", net.gradBias)):
+        _check(got, want[name], name)
+    assert torch.equal(net.state[0], h0[0]) and torch.equal(net.gradState[5], gh[5])
+
+
+@pytest.mark.gpu
+def test_tokens_one_after_the_other():
+    net, x, gate, _, h0, _ = _data(5, 40, 300, torch.bfloat16, 8)
+    want = _plain(x, gate, net.bias, h0)
+    state = h0.clone()
+    for t in range(40):
+        y = net.step([x[:, t], gate[:, t]], state)
+        _check(y, (want["output"][0][:, t], want["output"][1][:, t]), t)
+    _check(state, want["state"], "state")
+    planes = x[:, :1].transpose(1, 2).contiguous().transpose(1, 2)
+    strided = torch.randn(5, 600, device="cuda").bfloat16()[:, ::2]     # channels two apart
+    a = net.step([strided, strided], h0.clone())
+    b = net.step([strided.contiguous(), strided.contiguous()], h0.clone())
+    assert torch.equal(a, b)
+    assert torch.equal(net.updateOutput([planes, gate[:, :1]], state=h0), net.updateOutput([x[:, :1], gate[:, :1]], state=h0))
+
+
+@pytest.mark.gpu
+def test_parts_continue_a_sequence():
+    """A sequence in two calls, the state handed on in its own place: bit for bit where the cut lies between tiles."""
+    net, x, gate, _, h0, _ = _data(2, 1024, 100, torch.float32, 9)
+    whole = net.updateOutput([x, gate], state=h0).clone()
+    last = net.state.clone()
+    first = net.updateOutput([x[:, :512], gate[:, :512]], state=h0).clone()
+    second = net.updateOutput([x[:, 512:], gate[:, 512:]], state=net.state)
+    want = _plain(x, gate, net.bias, h0)
+    _check(torch.cat((first, second), 1), want["output"], "output")
+    _check(net.state, want["state"], "state")
+    assert torch.equal(first, whole[:, :512]) and last.shape == net.state.shape
+
+
+@pytest.mark.gpu
+def test_no_steps_and_no_sequences():
+    net, x, gate, gy, h0, gh = _data(3, 4, 10, torch.float32, 10)
+    empty = x[:, :0]
+    assert net.updateOutput([empty, empty], state=h0).shape == (3, 0, 10) and torch.equal(net.state, h0)
+    net.backward([empty, empty], empty, gradState=gh)
+    assert torch.equal(net.gradState, gh) and bool((net.gradBias == 0).all())
+    net.updateOutput([empty, empty])
+    assert bool((net.state == 0).all())
+    net.gradBias.fill_(1.0)
+    none = x[:0]
+    assert net.updateOutput([none, none]).shape == (0, 4, 10)
+    net.backward([none, none], none)
+    assert bool((net.gradBias == 0).all())
+
+
+@pytest.mark.gpu
+def test_results_repeat_and_halves_match_the_whole():
+    """The state goes from tile to tile through memory in an order that changes from run to run; no result does."""
+    net, x, gate, gy, h0, gh = _data(2, 20000, 300, torch.bfloat16, 11)
+    results = lambda: [net.output, net.state, *net.gradInput, net.gradState, net.gradBias]   # noqa: E731
+    first = None
+    for rep in range(4):
+        net.updateOutput([x, gate], state=h0)
+        if rep == 3:
+            net.updateGradInput([x, gate], gy, gh)
+            net.gradBias.fill_(float("nan"))
+            net.accGradParameters([x, gate], gy, 1.0, gh)
+        else:
+            net.backward([x, gate], gy, gradState=gh)
+        now = [t.clone() for t in results()]
+        if first is None:
+            first = now
+            for t in results():
+                t.fill_(float("nan"))
+        for a, b in zip(first, now):
+            assert torch.equal(a, b), rep
+
+
+@pytest.mark.gpu
+def test_gates_open_and_closed():
+    net, x, gate, gy, h0, gh = _data(2, 300, 40, torch.float32, 12)
+    gate[0, 5], gate[0, 6], gate[1, 7], gate[1, 8] = float("inf"), -float("inf"), 300.0, -300.0
+    y = net.updateOutput([x, gate], state=h0)
+    net.backward([x, gate], gy, gradState=gh)
+    assert torch.equal(y[0, 5], y[0, 4]) and torch.equal(y[1, 7], y[1, 6])       # kept
+    for b, t in ((0, 6), (1, 8)):                                                # replaced: h + (x - h), two roundings
+        assert bool(((y[b, t] - x[b, t]).abs() <= 2 * U * (x[b, t].abs() + y[b, t - 1].abs())).all())
+    for t in (y, net.state, *net.gradInput, net.gradState, net.gradBias):
+        assert bool(t.isfinite().all())
+    x[0, 100, 3] = float("nan")                                                  # reaches what follows in its channel alone
+    y2 = net.updateOutput([x, gate], state=h0)
+    bad = torch.zeros(2, 300, 40, dtype=torch.bool, device="cuda")
+    bad[0, 100:, 3] = True
+    assert torch.equal(y2.isnan(), bad)
+
+
+@pytest.mark.gpu
+def test_gradient_against_differences():
+    """Directional derivative by central differences in 32 bits; the bound is the rounding of the outputs over the step
+    and how far the same difference in 64 bits is from the gradient in 64 bits."""
+    h = 2.0 ** -5
+    net, x, gate, gy, h0, gh = _data(2, 150, 6, torch.float32, 13)
+    _, dx, dz, _, dh, _ = _data(2, 150, 6, torch.float32, 14)
+    net.updateOutput([x, gate], state=h0)
+    net.backward([x, gate], gy, gradState=gh)
+    dot = lambda a, b: float((a.detach().cpu().double() * b.detach().cpu().double()).sum())   # noqa: E731
+    mine = dot(net.gradInput[0], dx) + dot(net.gradInput[1], dz) + dot(net.gradState, dh)
+    want = _plain(x, gate, net.bias, h0, None, gy, gh)
+    exact = dot(want["gradX"][0], dx) + dot(want["gradGate"][0], dz) + dot(want["gradState"][0], dh)
+    tol = dot(want["gradX"][1], dx.abs()) + dot(want["gradGate"][1], dz.abs()) + dot(want["gradState"][1], dh.abs())
+    sums, plain = [], []
+    for sign in (1, -1):
+        at = [x + sign * h * dx, gate + sign * h * dz]
+        y = net.updateOutput(at, state=h0 + sign * h * dh)
+        ref = _plain(*at, net.bias, h0 + sign * h * dh)
+        sums.append(dot(y, gy) + dot(net.state, gh))
+        plain.append(dot(ref["output"][0], gy) + dot(ref["state"][0], gh))
+        tol += (dot(ref["output"][1] + U * ref["output"][0].abs(), gy.abs()) + dot(ref["state"][1], gh.abs())) / (2 * h)
+    tol += 1.01 * abs((plain[0] - plain[1]) / (2 * h) - exact) + 1e-6 * abs(exact)
+    assert abs((sums[0] - sums[1]) / (2 * h) - mine) <= tol
+    assert tol < 0.1 * abs(exact)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [100, 1500])
+def test_replays_from_a_graph(T):
+    net, x, gate, gy, h0, gh = _data(2, T, 200, torch.bfloat16, 15)
+    other, *_ = _data(2, T, 200, torch.bfloat16, 15)
+
+    def step(m):
+        m.updateOutput([x, gate], state=h0)
+        m.backward([x, gate], gy, gradState=gh)
+
+    results = lambda m: [m.output, m.state, *m.gradInput, m.gradState, m.gradBias]   # noqa: E731
+    step(net)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(net)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(net)
+    for rep in range(3):
+        x.mul_(-0.5)
+        for t in results(net):
+            t.fill_(float("nan"))
+        (x.float() * 2).sum().item()
+        graph.replay()
+        torch.cuda.synchronize()
+        step(other)
+        for a, b in zip(results(net), results(other)):
+            assert torch.equal(a, b), rep
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once():
+    """Two long recurrences, each with its workspace, on two streams: neither waits for the other's tiles."""
+    jobs = [_data(2, 30000, 200, torch.bfloat16, 16 + i) for i in range(2)]
+    want = []
+    for net, x, gate, gy, h0, gh in jobs:
+        net.updateOutput([x, gate], state=h0)
+        net.backward([x, gate], gy, gradState=gh)
+        want.append([t.clone() for t in (net.output, *net.gradInput, net.gradBias)])
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in jobs]
+    for rep in range(3):
+        for s, (net, x, gate, gy, h0, gh) in zip(streams, jobs):
+            with torch.cuda.stream(s):
+                net.updateOutput([x, gate], state=h0)
+                net.backward([x, gate], gy, gradState=gh)
+    torch.cuda.synchronize()
+    for (net, *_), w in zip(jobs, want):
+        for a, b in zip((net.output, *net.gradInput, net.gradBias), w):
+            assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """2.3 thousand million elements: the last tiles from the checkpoint before them, as a sequence of their own."""
+    T, D = 70016, 32768
+    from fbcunn_amd import nn
+    gen = torch.Generator("cuda").manual_seed(1)
+    x, gate = (torch.empty(1, T, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    net = nn.GatedLinearRecurrence(D)
+    net.bias.fill_(2.0)
+    y = net.updateOutput([x, gate])
+    kept = net._forward[3].view(torch.float32)[:T // 128 * D].view(-1, D)
+    part = nn.GatedLinearRecurrence(D)
+    part.bias.fill_(2.0)
+    for cut in (128 * 300, T - 256):
+        z = part.updateOutput([x[:, cut:cut + 256], gate[:, cut:cut + 256]], state=kept[cut // 128].view(1, D).contiguous())
+        assert torch.equal(z, y[:, cut:cut + 256])
+    net.backward([x, gate], y)
+    part.backward([x[:, T - 256:], gate[:, T - 256:]], y[:, T - 256:])
+    assert torch.equal(net.gradInput[1][:, T - 256:], part.gradInput[1])
+
+
+@pytest.mark.gpu
+def test_module_refusals():
+    from fbcunn_amd import nn
+    net = nn.GatedLinearRecurrence(8)
+    x = torch.randn(2, 5, 8, device="cuda")
+    ok = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    for call, error in ((lambda: net.updateOutput([x]), ValueError), (lambda: net.updateOutput([x, x[:1]]), ValueError),
+                        (lambda: net.updateOutput([x, x.half()]), TypeError), (lambda: net.updateOutput([x.cpu(), x]), TypeError),
+                        (lambda: net.updateOutput([x[..., :4]] * 2), ValueError), (lambda: net.updateOutput([x[0]] * 2), ValueError),
+                        (lambda: net.updateOutput([x, x], state=torch.zeros(2, 7, device="cuda")), ValueError),
+                        (lambda: net.updateOutput([x, x], state=torch.zeros(2, 8, device="cuda").half()), TypeError),
+                        (lambda: net.updateOutput([x, x], lengths=ok.long()), TypeError),
+                        (lambda: net.updateOutput([x, x], lengths=ok[:1]), ValueError),
+                        (lambda: net.updateOutput([x, x], lengths=ok.cpu()), TypeError),
+                        (lambda: net.backward([x, x], x), ValueError),
+                        (lambda: net.step([x, x], torch.zeros(2, 8, device="cuda")), ValueError),
+                        (lambda: net.step([x[:, 0], x[:, 0]], None), TypeError)):
+        with pytest.raises(error):
+            call()
+    net.updateOutput([x, x], lengths=ok)
+    with pytest.raises(ValueError):
+        net.backward([x[:1], x[:1]], x[:1])
+    net.evaluate()
+    net.updateOutput([x, x])
+    with pytest.raises(ValueError):
+        net.backward([x, x], x)
