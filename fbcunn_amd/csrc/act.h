@@ -55,10 +55,39 @@ __device__ __forceinline__ void store_some(T *p, Vec<T, N> v, long n)
         if (i < n) ((FBFC_GLOBAL T *)p)[i] = v[i];
 }
 
-// sigmoid(z) and sigmoid(-z) = 1 - sigmoid(z), each to its own precision however close the other is to one.
+// 16 bytes of a row of `channels` values, from place c on.  A load that would pass the row's end is moved back to end there,
+// so that no load has a condition (one would make the wavefront wait for the loads before it); end_of_row() then moves the
+// values to their places.
+template <typename T>
+__device__ __forceinline__ Vec<T, 16 / sizeof(T)> load_in_row(const T *row, int c, int channels)
+{
+    constexpr int V = 16 / sizeof(T);
+    if (channels < V) return load_some<V>(row + c, channels - c);  // the same for all lanes
+    return load_vec<V>(row + (c + V <= channels ? c : channels - V));
+}
+template <typename T>
+__device__ __forceinline__ void end_of_row(Vec<T, 16 / sizeof(T)> &v, int c, int channels)
+{
+    constexpr int V = 16 / sizeof(T);
+    if (channels < V) return;
+    const int over = c + V - channels, bits = (over < 0 ? 0 : over > V ? V : over) * 8 * (int)sizeof(T);
+    unsigned long w[2];
+    __builtin_memcpy(w, &v, 16);
+    if (bits >= 64) {
+        w[0] = bits == 128 ? 0 : w[1] >> (bits & 63);
+        w[1] = 0;
+    } else if (bits > 0) {
+        w[0] = w[0] >> bits | w[1] << (64 - bits);
+        w[1] >>= bits;
+    }
+    __builtin_memcpy(&v, w, 16);
+}
+
+// sigmoid(z) and sigmoid(-z) = 1 - sigmoid(z), each to its own precision however close the other is to one.  The
+// reciprocal is the hardware's, off by one unit.
 __device__ __forceinline__ void sigmoid_pair(float z, float &yes, float &no)
 {
-    const float e = __expf(-fabsf(z)), r = 1.0f / (1.0f + e);
+    const float e = __expf(-fabsf(z)), r = __builtin_amdgcn_rcpf(1.0f + e);
     yes = z < 0.0f ? e * r : r;
     no = z < 0.0f ? r : e * r;
 }

@@ -19,39 +19,45 @@
 #include <hip/hip_runtime.h>
 
 #include <cmath>
+#include <type_traits>
 
 #include "kernels.h"
+#include "lanes.h"
 #include "training.h"
 
 namespace fbfc {
 
 constexpr int kMaxGroups = 2048;   // 8 workgroups on each of 256 CUs
+constexpr int kStretch = 4;        // vectors of 4 parameters that a lane holds at once
+typedef float float4v __attribute__((ext_vector_type(4)));
+typedef float float2v __attribute__((ext_vector_type(2)));
 constexpr unsigned kHash1 = 0x9E3779B1u, kHash2 = 0xBB67AE85u, kHash3 = 0xB504F335u;  // fractions of the golden
                                                                                       // ratio, of the roots of 3 and 1/2, odd
 
-static __host__ __device__ AdamwClock clock_at(long t, double beta1, double beta2, unsigned seed)
+// The powers of the betas are carried along by one product a step: no logarithm at the end of a step.
+static __host__ __device__ AdamwClock clock_of(long t, double power1, double power2, unsigned seed)
 {
     AdamwClock c;
-    const double next = (double)(t + 1);
     c.t = t;
-    c.inv_bias1 = 1.0 / -expm1(next * log(beta1));
-    c.inv_root2 = (float)(1.0 / sqrt(-expm1(next * log(beta2))));
+    c.power1 = power1;
+    c.power2 = power2;
+    c.inv_bias1 = 1.0 / (1.0 - power1);
+    c.inv_root2 = (float)(1.0 / sqrt(1.0 - power2));
     c.key = seed * kHash1 + (unsigned)(t + 1) * kHash2;
     c.done = 0;
     return c;
 }
 
-AdamwClock adamw_clock(long t, double beta1, double beta2, unsigned seed) { return clock_at(t, beta1, beta2, seed); }
-
-__global__ void adamw_set_clock_kernel(AdamwClock *clock, long t, double beta1, double beta2, unsigned seed)
+AdamwClock adamw_clock(long t, double beta1, double beta2, unsigned seed)
 {
-    *clock = clock_at(t, beta1, beta2, seed);
+    return clock_of(t, std::pow(beta1, (double)(t + 1)), std::pow(beta2, (double)(t + 1)), seed);
 }
 
-// Two 20-bit numbers in the upper bits of `a` and `b`.
-__device__ __forceinline__ void random_pair(long i, unsigned key, unsigned &a, unsigned &b)
+__global__ void adamw_set_clock_kernel(AdamwClock *clock, AdamwClock to) { *clock = to; }
+
+// Two 20-bit numbers, of the place whose product with kHash1, plus the key, is `x`.
+__device__ __forceinline__ void random_pair(unsigned x, unsigned &a, unsigned &b)
 {
-    unsigned x = (unsigned)i * kHash1 + (unsigned)((unsigned long)i >> 32) * kHash3 + key;
     x ^= x >> 16;
     x *= kHash2;
     x ^= x >> 15;
@@ -64,26 +70,23 @@ __device__ __forceinline__ void random_pair(long i, unsigned key, unsigned &a, u
     b = y >> 12;
 }
 
-// The largest value of the wavefront; NaN if one is NaN.
-__device__ __forceinline__ float wave_max(float v)
+// The largest magnitude of the wavefront.  The bits of magnitudes are in the order of their values, a NaN's above all.
+__device__ __forceinline__ float wave_top(const float4v &v)
 {
+    unsigned m[4];
 #pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-        const float o = __shfl_xor(v, off, 64);
-        v = (o > v || o != o) ? o : v;
-    }
-    return v;
+    for (int i = 0; i < 4; ++i) m[i] = __float_as_uint(v[i]) & 0x7FFFFFFFu;
+    const unsigned top = max(max(m[0], m[1]), max(m[2], m[3]));
+    return __uint_as_float(lanes_reduce<64>(top, [](unsigned a, unsigned b) { return max(a, b); }));
 }
-__device__ __forceinline__ float max_nan(float a, float b) { return (b > a || b != b) ? b : a; }
 
-// e4m3 bits of four magnitudes times `inverse`.  The bits of a 32-bit float of 2^-120 times the value hold an e4m3
+// e4m3 bits of a magnitude times `inverse`.  The bits of a 32-bit float of 2^-120 times the value hold an e4m3
 // number on top (its smallest normal number, 2^-6, becomes the float's, 2^-126), so a 20-bit random number added below
 // rounds it, subnormal numbers too.
 __device__ __forceinline__ unsigned round8(float magnitude, float inverse, unsigned random)
 {
     const unsigned bits = __float_as_uint(magnitude * inverse * 0x1p-120f);
-    const unsigned code = (bits + random) >> 20;
-    return code < 0x7Eu ? code : 0x7Eu;
+    return min((bits + random) >> 20, 0x7Eu);
 }
 
 // scale of a block, and its inverse; a block below 2^-100 is zero
@@ -94,14 +97,89 @@ __device__ __forceinline__ float scale8(float top, float &inverse)
     return scale;
 }
 
-typedef float float4v __attribute__((ext_vector_type(4)));
-typedef float float2v __attribute__((ext_vector_type(2)));
-
-__device__ __forceinline__ float4v decode8(unsigned codes)
+__device__ __forceinline__ float4v decode8(unsigned codes, float scale)
 {
     const float2v lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, false);
     const float2v hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)codes, true);
-    return float4v{lo[0], lo[1], hi[0], hi[1]};
+    return float4v{lo[0] * scale, lo[1] * scale, hi[0] * scale, hi[1] * scale};
+}
+
+// What a lane reads for its 4 parameters.
+template <typename P, typename G, int BITS>
+struct Four {
+    Vec<P, 4> p;
+    Vec<G, 4> g;
+    typename std::conditional<BITS == 32, float4v, unsigned>::type m, v;
+    float ms, vs;
+};
+
+template <typename P, typename G, int BITS>
+__device__ __forceinline__ void load_four(Four<P, G, BITS> &f, const AdamwArgs &a, const P *param, const G *grad, long at, long left)
+{
+    f.p = load_some<4>(param, left);
+    f.g = load_some<4>(grad, left);
+    if constexpr (BITS == 32) {
+        f.m = *reinterpret_cast<const float4v *>(static_cast<const float *>(a.m) + at);
+        f.v = *reinterpret_cast<const float4v *>(static_cast<const float *>(a.v) + at);
+    } else {
+        f.m = static_cast<const unsigned *>(a.m)[at >> 2];
+        f.v = static_cast<const unsigned *>(a.v)[at >> 2];
+        f.ms = a.m_scale[at >> 8];
+        f.vs = a.v_scale[at >> 8];
+    }
+}
+
+template <typename P, typename G, int BITS>
+__device__ __forceinline__ void step_four(const Four<P, G, BITS> &f, const AdamwArgs &a, float root2, float step, unsigned key, P *param, long at,
+                                          long left)
+{
+    float4v m, v;
+    if constexpr (BITS == 32) {
+        m = f.m;
+        v = f.v;
+    } else {
+        m = decode8(f.m, f.ms);
+        v = decode8(f.v, f.vs);
+    }
+    Vec<P, 4> out;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float g = (float)f.g[i] * a.grad_scale;
+        m[i] = m[i] * a.keep1 + g * a.take1;
+        v[i] = v[i] * a.keep2 + g * g * a.take2;
+        float q;
+        if constexpr (BITS == 32)
+            q = m[i] / (sqrtf(v[i]) * root2 + a.eps);
+        else  // the arithmetic, not the memory, bounds this form: root and reciprocal to one unit each
+            q = m[i] * __builtin_amdgcn_rcpf(__builtin_amdgcn_sqrtf(v[i]) * root2 + a.eps);
+        out[i] = (P)((float)f.p[i] * a.decay - q * step);
+    }
+    store_some<4>(param, out, left);
+    if constexpr (BITS == 32) {
+        *reinterpret_cast<float4v *>(static_cast<float *>(a.m) + at) = m;
+        *reinterpret_cast<float4v *>(static_cast<float *>(a.v) + at) = v;
+    } else {
+        float mi, vi;
+        const float ms = scale8(wave_top(m), mi), vs = scale8(wave_top(v), vi);
+        const unsigned x = (unsigned)at * kHash1 + (unsigned)((unsigned long)at >> 32) * kHash3 + key;
+        unsigned mc = 0, vc = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            unsigned r, q;
+            random_pair(x + i * kHash1, r, q);
+            const unsigned c = round8(fabsf(m[i]), mi, r) | (m[i] < 0.0f ? 0x80u : 0u);
+            unsigned w = round8(v[i], vi, q);
+            w = v[i] > 0.0f && vi > 0.0f ? max(w, 1u) : w;
+            mc |= c << (8 * i);
+            vc |= w << (8 * i);
+        }
+        static_cast<unsigned *>(a.m)[at >> 2] = mc;
+        static_cast<unsigned *>(a.v)[at >> 2] = vc;
+        if ((threadIdx.x & 63) == 0) {
+            a.m_scale[at >> 8] = ms;
+            a.v_scale[at >> 8] = vs;
+        }
+    }
 }
 
 template <typename P, typename G, int BITS>
@@ -113,63 +191,20 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a)
         const AdamwPiece piece = a.pieces[k];
         P *param = static_cast<P *>(piece.param);
         const G *grad = static_cast<const G *>(piece.grad);
-        for (long o = threadIdx.x * 4; (o & ~255L) < piece.n; o += 1024) {  // whole wavefronts stay or leave
-            const long at = piece.first + o, left = piece.n - o;
-            float4v p, g, m, v;
-            {
-                const Vec<P, 4> pv = load_some<4>(param + o, left);
-                const Vec<G, 4> gv = load_some<4>(grad + o, left);
-                if (BITS == 32) {
-                    m = *reinterpret_cast<const float4v *>(static_cast<const float *>(a.m) + at);
-                    v = *reinterpret_cast<const float4v *>(static_cast<const float *>(a.v) + at);
-                } else {
-                    const unsigned mc = static_cast<const unsigned *>(a.m)[at >> 2];
-                    const unsigned vc = static_cast<const unsigned *>(a.v)[at >> 2];
-                    m = decode8(mc) * a.m_scale[at >> 8];
-                    v = decode8(vc) * a.v_scale[at >> 8];
-                }
+        long o = threadIdx.x * 4;
+        // whole stretches: the loads of all of it before the first store
+        for (; o - threadIdx.x * 4 + kStretch * 1024 <= piece.n; o += kStretch * 1024) {
+            Four<P, G, BITS> f[kStretch];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    p[i] = (float)pv[i];
-                    g[i] = (float)gv[i] * a.grad_scale;
-                }
-            }
+            for (int j = 0; j < kStretch; ++j) load_four<P, G, BITS>(f[j], a, param + o + j * 1024, grad + o + j * 1024, piece.first + o + j * 1024, 4);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                m[i] = m[i] * a.keep1 + g[i] * a.take1;
-                v[i] = v[i] * a.keep2 + g[i] * g[i] * a.take2;
-                const float d = sqrtf(v[i]) * now.inv_root2 + a.eps;
-                p[i] = p[i] * a.decay - m[i] / d * step;
-            }
-            Vec<P, 4> out;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] = (P)p[i];
-            store_some<4>(param + o, out, left);
-            if (BITS == 32) {
-                *reinterpret_cast<float4v *>(static_cast<float *>(a.m) + at) = m;
-                *reinterpret_cast<float4v *>(static_cast<float *>(a.v) + at) = v;
-            } else {
-                float mi, vi;
-                const float ms = scale8(wave_max(max_nan(max_nan(fabsf(m[0]), fabsf(m[1])), max_nan(fabsf(m[2]), fabsf(m[3])))), mi);
-                const float vs = scale8(wave_max(max_nan(max_nan(v[0], v[1]), max_nan(v[2], v[3]))), vi);
-                unsigned mc = 0, vc = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    unsigned r, q;
-                    random_pair(at + i, now.key, r, q);
-                    const unsigned c = round8(fabsf(m[i]), mi, r) | (m[i] < 0.0f ? 0x80u : 0u);
-                    unsigned w = round8(v[i], vi, q);
-                    w = w == 0 && v[i] > 0.0f && vi > 0.0f ? 1u : w;
-                    mc |= c << (8 * i);
-                    vc |= w << (8 * i);
-                }
-                static_cast<unsigned *>(a.m)[at >> 2] = mc;
-                static_cast<unsigned *>(a.v)[at >> 2] = vc;
-                if ((threadIdx.x & 63) == 0) {
-                    a.m_scale[at >> 8] = ms;
-                    a.v_scale[at >> 8] = vs;
-                }
-            }
+            for (int j = 0; j < kStretch; ++j)
+                step_four<P, G, BITS>(f[j], a, now.inv_root2, step, now.key, param + o + j * 1024, piece.first + o + j * 1024, 4);
+        }
+        for (; (o & ~255L) < piece.n; o += 1024) {  // whole wavefronts stay or leave
+            Four<P, G, BITS> f;
+            load_four<P, G, BITS>(f, a, param + o, grad + o, piece.first + o, piece.n - o);
+            step_four<P, G, BITS>(f, a, now.inv_root2, step, now.key, param + o, piece.first + o, piece.n - o);
         }
     }
     // Every wavefront of this workgroup has read the clock; the last workgroup of all moves it on, so a step replayed
@@ -177,12 +212,12 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a)
     __syncthreads();
     if (threadIdx.x == 0 &&
         __hip_atomic_fetch_add(&a.clock->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1)
-        *a.clock = clock_at(now.t + 1, a.beta1, a.beta2, a.seed);
+        *a.clock = clock_of(now.t + 1, now.power1 * a.beta1, now.power2 * a.beta2, a.seed);
 }
 
 hipError_t launch_adamw_set_clock(const AdamwArgs &a, long t, hipStream_t s)
 {
-    FBFC_LAUNCH(adamw_set_clock_kernel, dim3(1), dim3(1), 0, s, a.clock, t, a.beta1, a.beta2, a.seed);
+    FBFC_LAUNCH(adamw_set_clock_kernel, dim3(1), dim3(1), 0, s, a.clock, adamw_clock(t, a.beta1, a.beta2, a.seed));
     return hipGetLastError();
 }
 

@@ -6,27 +6,33 @@
 
 namespace fbfc {
 
-template <int CTRL>
-__device__ __forceinline__ float lane_move(float v)
+template <int CTRL, typename T>
+__device__ __forceinline__ T lane_move(T v)
 {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xF, 0xF, true));
+    static_assert(sizeof(T) == 4, "32 bits a lane");
+    const int moved = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(T, moved);
 }
 
-template <int L, typename F>
-__device__ __forceinline__ float lanes_reduce(float v, F f)
+template <int L, typename T, typename F>
+__device__ __forceinline__ T lanes_reduce(T v, F f)
 {
     static_assert(L == 8 || L == 16 || L == 32 || L == 64, "groups of 8, 16, 32 or 64 lanes");
     v = f(v, lane_move<0xB1>(v));
     v = f(v, lane_move<0x4E>(v));
     v = f(v, lane_move<0x141>(v));
-    if (L >= 16) v = f(v, lane_move<0x140>(v));
-    if (L >= 32) {
-        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    if constexpr (L >= 16) v = f(v, lane_move<0x140>(v));
+    if constexpr (L >= 32) {
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const auto s = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const unsigned one = s[0], other = s[1];  // a bit cast of s[1] itself would read s[0]
+        v = f(__builtin_bit_cast(T, one), __builtin_bit_cast(T, other));
     }
-    if (L >= 64) {
-        const auto s = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
-        v = f(__uint_as_float(s[0]), __uint_as_float(s[1]));
+    if constexpr (L >= 64) {
+        const unsigned u = __builtin_bit_cast(unsigned, v);
+        const auto s = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const unsigned one = s[0], other = s[1];  // a bit cast of s[1] itself would read s[0]
+        v = f(__builtin_bit_cast(T, one), __builtin_bit_cast(T, other));
     }
     return v;
 }

@@ -19,6 +19,7 @@
 // gradients stay in registers too; these are then added over the workgroups in a fixed order by a second kernel.
 #include <hip/hip_runtime.h>
 
+#include "column_sums.h"
 #include "kernels.h"
 #include "lanes.h"
 #include "training.h"
@@ -69,8 +70,66 @@ __device__ __forceinline__ void load_row(Vec<T, kVec<T>> (&v)[E], const Rows &t,
 {
     const T *p = static_cast<const T *>(t.data) + row * t.stride;
 #pragma unroll
-    for (int e = 0; e < E; ++e) v[e] = load_some<kVec<T>>(p + c[e], channels - c[e]);
+    for (int e = 0; e < E; ++e) v[e] = load_in_row<T>(p, c[e], channels);
 }
+
+// The weights of this lane's channels: post scale, and pre; zero behind the last channel.
+template <int V, int E>
+__device__ __forceinline__ void load_weights(const NormArgs &a, bool branch, bool normed, const int (&c)[E], float (&post)[E * V], float (&pre)[E * V])
+{
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < V; i += 4) {
+            const int at = c[e] + i;
+            Vec<float, 4> p = {}, s = {}, q = {};
+            if (branch) {
+                p = load_some<4>(a.post + at, a.channels - at);
+                s = load_some<4>(a.scale + at, a.channels - at);
+            }
+            if (normed) q = load_some<4>(a.pre + at, a.channels - at);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                post[e * V + i + j] = p[j] * s[j];
+                pre[e * V + i + j] = q[j];
+            }
+        }
+}
+
+// Whether vector e of any lane of the wavefront passes the end of the rows.
+template <int V, int E>
+__device__ __forceinline__ unsigned ends_of(const int (&c)[E], int channels)
+{
+    unsigned ends = 0;
+#pragma unroll
+    for (int e = 0; e < E; ++e) ends |= __any(c[e] + V > channels) ? 1u << e : 0u;
+    return ends;
+}
+template <typename T, int E>
+__device__ __forceinline__ void end_row(Vec<T, kVec<T>> (&v)[E], unsigned ends, const int (&c)[E], int channels)
+{
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+        if (ends >> e & 1) end_of_row<T>(v[e], c[e], channels);
+}
+
+template <typename T, int E>
+struct ForwardRow {
+    Vec<T, kVec<T>> r[E], y[E], z[E];
+    __device__ __forceinline__ void load(const NormArgs &a, long row, const int (&c)[E])
+    {
+        load_row<T, E>(r, a.residual, row, c, a.channels);
+        if (a.branch.data != nullptr) load_row<T, E>(y, a.branch, row, c, a.channels);
+        if (a.gate.data != nullptr) load_row<T, E>(z, a.gate, row, c, a.channels);
+    }
+    __device__ __forceinline__ void end(unsigned ends, const int (&c)[E], int channels)
+    {
+        if (ends == 0) return;
+        end_row<T, E>(r, ends, c, channels);
+        end_row<T, E>(y, ends, c, channels);
+        end_row<T, E>(z, ends, c, channels);
+    }
+};
 
 template <typename T, int L, int E>
 __global__ __launch_bounds__(most_threads(L)) void norm_forward_kernel(NormArgs a)
@@ -82,21 +141,17 @@ __global__ __launch_bounds__(most_threads(L)) void norm_forward_kernel(NormArgs 
     int c[E];
     float post[E * V], pre[E * V];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-        c[e] = (walk.lane + e * walk.lanes) * V;
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const int at = c[e] + i;
-            post[e * V + i] = branch && at < a.channels ? a.post[at] * a.scale[at] : 0.0f;
-            pre[e * V + i] = normed && at < a.channels ? a.pre[at] : 0.0f;
-        }
-    }
+    for (int e = 0; e < E; ++e) c[e] = (walk.lane + e * walk.lanes) * V;
     const float share = 1.0f / (float)a.channels;
+    const unsigned ends = ends_of<V, E>(c, a.channels);
+    ForwardRow<T, E> in = {}, next = {};
+    if (walk.row < a.rows) next.load(a, walk.row, c);
+    load_weights<V, E>(a, branch, normed, c, post, pre);
     for (long row = walk.row; row < a.rows; row += walk.step) {
-        Vec<T, V> rv[E], yv[E] = {}, zv[E] = {};
-        load_row<T, E>(rv, a.residual, row, c, a.channels);
-        if (branch) load_row<T, E>(yv, a.branch, row, c, a.channels);
-        if (gated) load_row<T, E>(zv, a.gate, row, c, a.channels);
+        in = next;
+        if (row + walk.step < a.rows) next.load(a, row + walk.step, c);  // while this row is worked on
+        in.end(ends, c, a.channels);
+        const auto &rv = in.r, &yv = in.y, &zv = in.z;
         float r[E * V];
         if (branch) {
             float sum = 0.0f;
@@ -154,22 +209,15 @@ __global__ __launch_bounds__(most_threads(L)) void norm_backward_kernel(NormArgs
     constexpr bool kKeep = L != kWidest;
     int c[E];
     float post[N], pre[N], q[N], s[N];
-    auto weights = [&]() {
-#pragma unroll
-        for (int j = 0; j < N; ++j) {
-            const int at = c[j / V] + j % V;
-            post[j] = branch && at < a.channels ? a.post[at] * a.scale[at] : 0.0f;
-            pre[j] = normed && at < a.channels ? a.pre[at] : 0.0f;
-        }
-    };
 #pragma unroll
     for (int e = 0; e < E; ++e) c[e] = (walk.lane + e * walk.lanes) * V;
 #pragma unroll
     for (int j = 0; j < N; ++j) q[j] = s[j] = 0.0f;
-    if (kKeep) weights();
+    const unsigned ends = ends_of<V, E>(c, a.channels);
+    if (kKeep) load_weights<V, E>(a, branch, normed, c, post, pre);
     const float share = 1.0f / (float)a.channels;
     for (long row = walk.row; row < a.rows; row += walk.step) {
-        if (!kKeep) weights();
+        if (!kKeep) load_weights<V, E>(a, branch, normed, c, post, pre);
         Vec<T, V> rv[E] = {}, yv[E] = {}, zv[E] = {}, gv[E] = {}, nv[E] = {};
         if (normed) {
             load_row<T, E>(rv, a.residual, row, c, a.channels);
@@ -178,6 +226,13 @@ __global__ __launch_bounds__(most_threads(L)) void norm_backward_kernel(NormArgs
         if (branch) load_row<T, E>(yv, a.branch, row, c, a.channels);
         if (gated) load_row<T, E>(zv, a.gate, row, c, a.channels);
         if (a.grad_output.data != nullptr) load_row<T, E>(gv, a.grad_output, row, c, a.channels);
+        if (ends != 0) {
+            end_row<T, E>(rv, ends, c, a.channels);
+            end_row<T, E>(nv, ends, c, a.channels);
+            end_row<T, E>(yv, ends, c, a.channels);
+            end_row<T, E>(zv, ends, c, a.channels);
+            end_row<T, E>(gv, ends, c, a.channels);
+        }
         float i1 = 0.0f, k[N], g[N];
         if (branch) {
             float sum = 0.0f;
@@ -299,26 +354,19 @@ __global__ __launch_bounds__(most_threads(L)) void norm_backward_kernel(NormArgs
     }
 }
 
-// Adds the workgroups' sums: 16 channels and 16 slices of the workgroups a workgroup, in a fixed order.
-__global__ __launch_bounds__(256) void norm_weights_kernel(NormArgs a, int groups)
+// Adds the workgroups' sums.
+__global__ __launch_bounds__(kSumThreads) void norm_weights_kernel(NormArgs a, int groups)
 {
-    __shared__ float part[2][16][17];
-    const int i = threadIdx.x & 15, slice = threadIdx.x >> 4, at = blockIdx.x * 16 + i;
+    __shared__ float part[2][kSumSlices][kSumColumns];
+    const int at = blockIdx.x * kSumColumns + threadIdx.x % kSumColumns, slice = threadIdx.x / kSumColumns;
     float q = 0.0f, s = 0.0f;
-    if (at < a.channels)
-        for (int g = slice; g < groups; g += 16) {
-            const float *p = a.partial + (long)g * 2 * a.channels + at;
-            q += p[0];
-            s += p[a.channels];
-        }
-    part[0][slice][i] = q;
-    part[1][slice][i] = s;
-    __syncthreads();
-    if (slice != 0 || at >= a.channels) return;
-    for (int k = 1; k < 16; ++k) {
-        q += part[0][k][i];
-        s += part[1][k][i];
+    if (at < a.channels) {
+        q = slice_sum(a.partial + at, 2L * a.channels, groups, slice);
+        s = slice_sum(a.partial + a.channels + at, 2L * a.channels, groups, slice);
     }
+    q = slices_sum(q, part[0]);
+    s = slices_sum(s, part[1]);
+    if (threadIdx.x >= kSumColumns || at >= a.channels) return;
     if (a.grad_post != nullptr) a.grad_post[at] = q * a.scale[at] * a.factor;
     if (a.grad_scale != nullptr) a.grad_scale[at] = q * a.post[at] * a.factor;
     if (a.grad_pre != nullptr) a.grad_pre[at] = s * a.factor;
@@ -412,9 +460,9 @@ hipError_t launch_norm_backward(int type, const NormArgs &a, hipStream_t s)
         if (e != hipSuccess) return e;
     }
     if (a.grad_post == nullptr && a.grad_scale == nullptr && a.grad_pre == nullptr) return hipSuccess;
-    const int blocks = (a.channels + 15) / 16;
-    kernel_log_add("norm_weights_kernel", (long)blocks * 256);
-    FBFC_LAUNCH(norm_weights_kernel, dim3(blocks), dim3(256), 0, s, a, (int)r.groups);
+    const int blocks = (a.channels + kSumColumns - 1) / kSumColumns;
+    kernel_log_add("norm_weights_kernel", (long)blocks * kSumThreads);
+    FBFC_LAUNCH(norm_weights_kernel, dim3(blocks), dim3(kSumThreads), 0, s, a, (int)r.groups);
     return hipGetLastError();
 }
 

@@ -20,6 +20,9 @@
 // the forward pass leaves in `checkpoints` (4 bytes for 128 steps), so y is neither read nor relied on to have 32 bits.
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
+#include "column_sums.h"
 #include "kernels.h"
 #include "training.h"
 
@@ -28,6 +31,7 @@ namespace fbfc {
 constexpr int kRun = 16;      // steps of a wavefront
 constexpr int kWaves = 8;     // wavefronts of a workgroup, at most
 constexpr int kLanes = 64;
+constexpr float kLog2e = 1.44269504088896340736f;
 
 // Announcements.  A word is announced once it differs from what the workspace is filled with, all ones (a NaN that
 // announce() never writes), so value and flag arrive together and no fence is needed.
@@ -45,8 +49,8 @@ struct Chain {
 
 struct Shape {
     int waves, blocks;  // wavefronts of a workgroup, workgroups beside each other over the channels of a sequence
-    long tiles;         // after each other
-    long cols;          // batch * blocks
+    int tiles;          // after each other
+    int cols;           // batch * blocks
     bool chain;
 };
 
@@ -57,8 +61,8 @@ __host__ __device__ __forceinline__ Shape shape_of(int batch, int channels, long
     s.waves = runs < kWaves ? (int)runs : kWaves;
     if (s.waves < 1) s.waves = 1;
     s.blocks = (channels + kLanes * v - 1) / (kLanes * v);
-    s.tiles = (runs + s.waves - 1) / s.waves;
-    s.cols = (long)batch * s.blocks;
+    s.tiles = (int)((runs + s.waves - 1) / s.waves);  // recurrence_fits(): tiles * cols is below 2^31
+    s.cols = batch * s.blocks;
     // 512 workgroups fill the GPU by themselves; fewer leave CUs idle, and their tiles are then spread
     s.chain = s.tiles > 1 && s.cols < 512;
     return s;
@@ -69,7 +73,7 @@ __device__ __forceinline__ Chain chain_of(unsigned char *workspace, const Shape 
     Chain c;
     c.ticket = reinterpret_cast<unsigned *>(workspace);
     c.runs = reinterpret_cast<word64 *>(workspace + 256);
-    c.states = reinterpret_cast<unsigned *>(c.runs + s.tiles * s.cols * kLanes * v);
+    c.states = reinterpret_cast<unsigned *>(c.runs + (long)s.tiles * s.cols * kLanes * v);
     return c;
 }
 static size_t chain_bytes(const Shape &s, int v) { return 256 + (size_t)s.tiles * s.cols * kLanes * v * 12; }
@@ -81,15 +85,15 @@ __global__ __launch_bounds__(256) void recurrence_clear_kernel(uint4 *p, long n)
 
 // The state in front of tile `at` of column `col`, of this lane's channels; `dir` is where the tile before it lies.
 template <int V>
-__device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, long at, long col, int dir, int lane, float (&h)[V])
+__device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, int at, int col, int dir, int lane, float (&h)[V])
 {
-    const long cell = kLanes * V;
-    long j = at + dir;
+    const int cell = kLanes * V;
+    int j = at + dir;
     while (true) {
         bool state = true, run = true;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const long k = (j * s.cols + col) * cell + lane * V + i;
+            const long k = (long)(j * s.cols + col) * cell + lane * V + i;
             const unsigned p = __hip_atomic_load(ch.states + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             const word64 r = __hip_atomic_load(ch.runs + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             h[i] = __uint_as_float(p);
@@ -103,123 +107,215 @@ __device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, long 
     for (j -= dir; j != at; j -= dir) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            const word64 r = __hip_atomic_load(ch.runs + (j * s.cols + col) * cell + lane * V + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            const word64 r = __hip_atomic_load(ch.runs + (long)(j * s.cols + col) * cell + lane * V + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             h[i] = fmaf(__uint_as_float((unsigned)r), h[i], __uint_as_float((unsigned)(r >> 32)));
         }
     }
 }
 
 template <int V>
-__device__ __forceinline__ void announce_run(const Chain &ch, const Shape &s, long at, long col, int lane, const float (&A)[V], const float (&S)[V])
+__device__ __forceinline__ void announce_run(const Chain &ch, const Shape &s, int at, int col, int lane, const float (&A)[V], const float (&S)[V])
 {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        __hip_atomic_store(ch.runs + (at * s.cols + col) * (kLanes * V) + lane * V + i,
+        __hip_atomic_store(ch.runs + (long)(at * s.cols + col) * (kLanes * V) + lane * V + i,
                            (word64)announced(S[i]) << 32 | announced(A[i]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 template <int V>
-__device__ __forceinline__ void announce_state(const Chain &ch, const Shape &s, long at, long col, int lane, const float (&h)[V])
+__device__ __forceinline__ void announce_state(const Chain &ch, const Shape &s, int at, int col, int lane, const float (&h)[V])
 {
 #pragma unroll
     for (int i = 0; i < V; ++i)
-        __hip_atomic_store(ch.states + (at * s.cols + col) * (kLanes * V) + lane * V + i, announced(h[i]), __ATOMIC_RELAXED,
+        __hip_atomic_store(ch.states + (long)(at * s.cols + col) * (kLanes * V) + lane * V + i, announced(h[i]), __ATOMIC_RELAXED,
                            __HIP_MEMORY_SCOPE_AGENT);
 }
 
-// V channels of this lane in one row of a tensor.  The address is moved back where the row ends inside or before it, and
-// the values are moved to their places, so that no load has a condition.
-template <typename T, int V>
-struct LaneRow {
-    const T *base;
-    long st, off;
-    int shift;
-    __device__ LaneRow(const Steps &t, int b, int c, int channels)
+// A tensor's rows as a lane reads and writes them: V channels from c on.  Where the last block of channels ends inside
+// or before a lane, its loads are moved back to end with the row, so that no load has a condition, and an odd last channel
+// is then moved to its place.  DENSE: channels side by side, with an offset that fits 32 bits, so that the row's
+// address stays in scalar registers.
+template <typename T, bool DENSE>
+constexpr int kLaneChannels = DENSE && sizeof(T) == 2 ? 2 : 1;  // 4 bytes a lane
+
+template <typename T, bool DENSE>
+struct LaneRows {
+    static constexpr int V = kLaneChannels<T, DENSE>;
+    typedef typename std::conditional<DENSE, unsigned, long>::type Offset;
+    const char *base;
+    long st;             // bytes from row to row
+    Offset off;          // of this lane's loads in a row, in bytes
+    __device__ LaneRows(const Steps &t, int b, int c, int channels)
     {
-        base = static_cast<const T *>(t.data) + (long)b * t.sb;
-        st = t.st;
+        base = static_cast<const char *>(t.data) + (long)b * t.sb * (long)sizeof(T);
+        st = t.st * (long)sizeof(T);
         const int first = c + V <= channels ? c : channels - V;
-        shift = c - first;
-        off = (long)first * t.sc;
+        off = (Offset)(DENSE ? (long)first * (long)sizeof(T) : first * t.sc * (long)sizeof(T));
     }
-    __device__ __forceinline__ Vec<T, V> load(long step) const { return load_vec<V>(base + step * st + off); }
-    __device__ __forceinline__ float value(const Vec<T, V> &v, int i) const
+    __device__ __forceinline__ const char *row(long step) const
     {
-        if (V == 1) return (float)v[0];
-        return (float)(i == 0 && shift == 1 ? v[1] : v[i]);
+        const unsigned long at = (unsigned long)(base + step * st);
+        const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)at), hi = __builtin_amdgcn_readfirstlane((unsigned)(at >> 32));
+        return reinterpret_cast<const char *>((unsigned long)hi << 32 | lo);
+    }
+    // Where the lane's values lie in a row.  The row's address is kept by itself, in scalar registers: it would else be
+    // added up in two registers of every lane for each row.
+    __device__ __forceinline__ T *place(const char *row) const
+    {
+        Offset o = off;
+        if constexpr (DENSE) asm("" : "+s"(row), "+v"(o));
+        return reinterpret_cast<T *>(const_cast<char *>(row) + o);
+    }
+    // 16 rows from step t0 on, of which `n` are the sequence's; the others repeat its last one (there is one).  FULL: all are
+    // the sequence's, and all lanes have V channels.
+    template <bool FULL>
+    __device__ __forceinline__ void load(Vec<T, V> (&v)[kRun], long t0, int n, long len, int c, int channels) const
+    {
+        const char *r = row(FULL || n > 0 ? t0 : len - 1);
+#pragma unroll
+        for (int t = 0; t < kRun; ++t) {
+            v[t] = load_vec<V>(place(r));
+            r += FULL || t + 1 < n ? st : 0;
+        }
+        if (FULL) return;
+        if constexpr (V == 2)
+            if (__any(c + 1 == channels))
+#pragma unroll
+                for (int t = 0; t < kRun; ++t) v[t][0] = c + 1 == channels ? v[t][1] : v[t][0];
+    }
+    template <bool FULL>
+    __device__ __forceinline__ void store(const char *row, int c, int channels, const float (&x)[V]) const
+    {
+        T *p = place(row);
+        Vec<T, V> o;
+#pragma unroll
+        for (int i = 0; i < V; ++i) o[i] = (T)x[i];
+        if (FULL || c + V <= channels) store_vec<V>(p, o);
+        else if (V == 2 && c < channels) store_vec<1>(p + 1, Vec<T, 1>{o[0]});  // its address was moved back by one
     }
 };
+
+// The same value, of which the compiler knows nothing: what was computed from it before is not kept in registers for what
+// follows.
 template <typename T, int V>
-__device__ __forceinline__ void store_lane(const Steps &t, int b, long step, int c, int channels, const float (&x)[V])
+__device__ __forceinline__ void forget(Vec<T, V> &v)
 {
-    T *p = static_cast<T *>(t.data) + (long)b * t.sb + step * t.st + (long)c * t.sc;
-    Vec<T, V> o;
-#pragma unroll
-    for (int i = 0; i < V; ++i) o[i] = (T)x[i];
-    if (c < channels) store_some<V>(p, o, channels - c);
+    if constexpr (sizeof(T) * V == 4) {
+        unsigned u = __builtin_bit_cast(unsigned, v);
+        asm("" : "+v"(u));
+        v = __builtin_bit_cast(Vec<T, V>, u);
+    }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(kLanes *kWaves) void recurrence_forward_kernel(RecArgs a)
+// 1 - a = 1 / (1 + e^z), with e^z = 2^(gate log2 e + bias2); e^z itself in `e`.
+__device__ __forceinline__ float closed(float gate, float bias2, float &e)
 {
+    e = __builtin_amdgcn_exp2f(fmaf(gate, kLog2e, bias2));
+    return __builtin_amdgcn_rcpf(1.0f + e);
+}
+
+// Where a workgroup works: its column (sequence and block of channels) and the tiles it walks over.
+struct Place {
+    int col, order;     // order: which of the column's tiles, counted in the order in which they depend on each other
+    int b, c;
+    long len;           // steps of the sequence
+};
+template <int V>
+__device__ __forceinline__ Place place_of(const int *lengths, long steps, const Shape &s, const Chain &ch, unsigned *given)
+{
+    unsigned work = blockIdx.x;
+    if (s.chain) {
+        if (threadIdx.x == 0) *given = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+        __syncthreads();
+        work = __builtin_amdgcn_readfirstlane(*given);
+    }
+    Place p;
+    p.order = __builtin_amdgcn_readfirstlane(work / (unsigned)s.cols);
+    p.col = __builtin_amdgcn_readfirstlane(work % (unsigned)s.cols);
+    p.b = p.col / s.blocks;
+    p.c = p.col % s.blocks * kLanes * V + (threadIdx.x & 63) * V;
+    p.len = steps;
+    if (lengths != nullptr) {
+        const long n = __builtin_amdgcn_readfirstlane(lengths[p.b]);
+        p.len = n < 0 ? 0 : n < p.len ? n : p.len;
+    }
+    return p;
+}
+
+// How many of the 16 steps from t0 on lie before `end`.
+__device__ __forceinline__ int steps_before(long t0, long end) { return (int)(end - t0 < 0 ? 0 : end - t0 < kRun ? end - t0 : kRun); }
+
+// Zero in the steps behind the end.
+template <typename T, int V>
+__device__ __forceinline__ void cut_run(Vec<T, V> (&v)[kRun], int n)
+{
+#pragma unroll
+    for (int t = 0; t < kRun; ++t)
+        if (t >= n) v[t] = Vec<T, V>{};
+}
+
+template <typename T, bool DENSE>
+__global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(RecArgs a)
+{
+    constexpr int V = kLaneChannels<T, DENSE>;
     __shared__ float sA[2][kWaves][kLanes * V], sS[2][kWaves][kLanes * V], carried[kLanes * V];
     __shared__ unsigned given;
-    const Shape s = shape_of(a.batch, a.channels, a.steps, V);
+    const long steps = a.steps;
+    const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    long work = blockIdx.x;
-    if (s.chain) {
-        if (threadIdx.x == 0) given = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-        __syncthreads();
-        work = __builtin_amdgcn_readfirstlane(given);
-    }
-    const long col = work % s.cols;
-    const int b = (int)(col / s.blocks), c = (int)(col % s.blocks) * kLanes * V + lane * V;
-    const long first = s.chain ? work / s.cols : 0, end = s.chain ? first + 1 : s.tiles;
-    long len = a.steps;
-    if (a.lengths != nullptr) {
-        const long n = a.lengths[b];
-        len = n < 0 ? 0 : n < len ? n : len;
-    }
-    const LaneRow<T, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels);
-    float bias[V], carry[V];  // carry: wavefront 0, the state before the tile
+    const Place p = place_of<V>(a.lengths, steps, s, ch, &given);
+    const long len = p.len;
+    const int col = p.col, end = s.chain ? p.order + 1 : s.tiles, b = p.b, c = p.c;
+    const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
+    float bias2[V], carry[V];  // carry: wavefront 0, the state before the tile
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        bias[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] : 0.0f;
+        bias2[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] * kLog2e : 0.0f;
         carry[i] = a.state_in != nullptr && c + i < a.channels ? a.state_in[(long)b * a.channels + c + i] : 0.0f;
     }
+    const bool whole = __all(c + V <= a.channels);
     int turn = 0;
-    for (long tile = first; tile < end; ++tile, turn ^= 1) {
-        const long t0 = (tile * s.waves + w) * kRun;
-        float x[kRun][V], k[kRun][V], A[V], S[V];  // k: 1 - a
-        if (len > 0) {
-            Vec<T, V> xv[kRun], gv[kRun];
-#pragma unroll
-            for (int t = 0; t < kRun; ++t) {
-                const long at = t0 + t < len ? t0 + t : len - 1;
-                xv[t] = xr.load(at);
-                gv[t] = gr.load(at);
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) A[i] = 1.0f, S[i] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < kRun; ++t) {
-                const bool live = t0 + t < len;
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float keep;
-                    sigmoid_pair(gr.value(gv[t], i) + bias[i], keep, k[t][i]);
-                    x[t][i] = live ? xr.value(xv[t], i) : 0.0f;
-                    k[t][i] = live ? k[t][i] : 0.0f;
-                    A[i] *= live ? keep : 1.0f;
-                    S[i] = fmaf(k[t][i], x[t][i] - S[i], S[i]);
-                }
-            }
-        } else {
+    for (int tile = p.order; tile < end; ++tile, turn ^= 1) {
+        const long t0 = ((long)__builtin_amdgcn_readfirstlane(tile) * s.waves + w) * kRun;
+        const int n = steps_before(t0, len), n_all = steps_before(t0, steps);
+        const bool full = n == kRun && whole;
+        Vec<T, V> x[kRun];
+        float k[kRun][V], A[V], S[V];  // k: 1 - a
+        auto read = [&](auto all) {
+            constexpr bool FULL = decltype(all)::value;
+            Vec<T, V> gate[kRun];
+            xr.template load<FULL>(x, t0, n, len, c, a.channels);
+            gr.template load<FULL>(gate, t0, n, len, c, a.channels);
+            if (!FULL && n < kRun) cut_run<T, V>(x, n);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                A[i] = 1.0f, S[i] = 0.0f;
+                A[i] = 1.0f;
+                S[i] = 0.0f;
 #pragma unroll
-                for (int t = 0; t < kRun; ++t) x[t][i] = k[t][i] = 0.0f;
+                for (int t = 0; t < kRun; ++t) {
+                    float e;
+                    k[t][i] = closed((float)gate[t][i], bias2[i], e);
+                    if (!FULL && t >= n) k[t][i] = 0.0f;
+                    A[i] = fmaf(-k[t][i], A[i], A[i]);
+                    S[i] = fmaf(k[t][i], (float)x[t][i] - S[i], S[i]);
+                }
+            }
+        };
+        if (full) {
+            read(std::true_type{});
+        } else if (len > 0) {
+            read(std::false_type{});
+        } else {
+#pragma unroll
+            for (int t = 0; t < kRun; ++t) {
+                x[t] = Vec<T, V>{};
+#pragma unroll
+                for (int i = 0; i < V; ++i) k[t][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                A[i] = 1.0f;
+                S[i] = 0.0f;
             }
         }
 #pragma unroll
@@ -240,14 +336,17 @@ __global__ __launch_bounds__(kLanes *kWaves) void recurrence_forward_kernel(RecA
                 if (tile + 1 < s.tiles) announce_run<V>(ch, s, tile, col, lane, A, S);
                 look_back<V>(ch, s, tile, col, -1, lane, carry);
             }
+            float after[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) after[i] = fmaf(A[i], carry[i], S[i]);
+            if (s.chain && tile + 1 < s.tiles) announce_state<V>(ch, s, tile, col, lane, after);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 carried[lane * V + i] = carry[i];
                 if (a.checkpoints != nullptr && c + i < a.channels)
-                    a.checkpoints[(tile * a.batch + b) * a.channels + c + i] = carry[i];
-                carry[i] = fmaf(A[i], carry[i], S[i]);
+                    a.checkpoints[((long)tile * a.batch + b) * a.channels + c + i] = carry[i];
+                carry[i] = after[i];
             }
-            if (s.chain && tile + 1 < s.tiles) announce_state<V>(ch, s, tile, col, lane, carry);
         }
         __syncthreads();
         float h[V];
@@ -257,15 +356,23 @@ __global__ __launch_bounds__(kLanes *kWaves) void recurrence_forward_kernel(RecA
 #pragma unroll
             for (int i = 0; i < V; ++i) h[i] = fmaf(sA[turn][j][lane * V + i], h[i], sS[turn][j][lane * V + i]);
 #pragma unroll
-        for (int t = 0; t < kRun; ++t) {
-            float out[V];
+        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]);
+        auto write = [&](auto all) {
+            constexpr bool FULL = decltype(all)::value;
+            const char *to = yr.row(t0);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                h[i] = fmaf(k[t][i], x[t][i] - h[i], h[i]);
-                out[i] = t0 + t < len ? h[i] : 0.0f;
+            for (int t = 0; t < kRun; ++t, to += yr.st) {
+                float out[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    h[i] = fmaf(k[t][i], (float)x[t][i] - h[i], h[i]);
+                    out[i] = FULL || t < n ? h[i] : 0.0f;
+                }
+                if (FULL || t < n_all) yr.template store<FULL>(to, c, a.channels, out);
             }
-            if (t0 + t < a.steps) store_lane<T, V>(a.y, b, t0 + t, c, a.channels, out);
-        }
+        };
+        if (full) write(std::true_type{});
+        else write(std::false_type{});
         if (a.state_out != nullptr && tile + 1 == s.tiles && w + 1 == s.waves)
 #pragma unroll
             for (int i = 0; i < V; ++i)
@@ -273,83 +380,89 @@ __global__ __launch_bounds__(kLanes *kWaves) void recurrence_forward_kernel(RecA
     }
 }
 
-template <typename T, int V>
-__global__ __launch_bounds__(kLanes *kWaves) void recurrence_backward_kernel(RecArgs a, float *partial)
+template <typename T, bool DENSE>
+__global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(RecArgs a, float *partial)
 {
+    constexpr int V = kLaneChannels<T, DENSE>;
     __shared__ float sA[2][kWaves][kLanes * V], sS[2][kWaves][kLanes * V], sR[2][kWaves][kLanes * V], carried[kLanes * V];
     __shared__ unsigned given;
-    const Shape s = shape_of(a.batch, a.channels, a.steps, V);
+    const long steps = a.steps;
+    const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    long work = blockIdx.x;
-    if (s.chain) {
-        if (threadIdx.x == 0) given = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-        __syncthreads();
-        work = __builtin_amdgcn_readfirstlane(given);
-    }
-    const long col = work % s.cols;
-    const int b = (int)(col / s.blocks), c = (int)(col % s.blocks) * kLanes * V + lane * V;
-    const long first = s.chain ? s.tiles - 1 - work / s.cols : s.tiles - 1, end = s.chain ? first : 0;
-    long len = a.steps;
-    if (a.lengths != nullptr) {
-        const long n = a.lengths[b];
-        len = n < 0 ? 0 : n < len ? n : len;
-    }
-    const LaneRow<T, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
-    float bias[V], carry[V];  // carry: wavefront 0, a_{t+1} u_{t+1} behind the tile
+    const Place p = place_of<V>(a.lengths, steps, s, ch, &given);
+    const long len = p.len;
+    const int col = p.col, first = s.tiles - 1 - p.order, end = s.chain ? first : 0, b = p.b, c = p.c;
+    const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
+        gxr(a.grad_x, b, c, a.channels), ggr(a.grad_gate, b, c, a.channels);
+    float bias2[V], carry[V];  // carry: wavefront 0, a_{t+1} u_{t+1} behind the tile
 #pragma unroll
     for (int i = 0; i < V; ++i) {
-        bias[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] : 0.0f;
+        bias2[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] * kLog2e : 0.0f;
         carry[i] = a.state_in != nullptr && c + i < a.channels ? a.state_in[(long)b * a.channels + c + i] : 0.0f;
     }
+    const bool whole = __all(c + V <= a.channels);
     int turn = 0;
-    for (long tile = first; tile >= end; --tile, turn ^= 1) {
-        const long t0 = (tile * s.waves + w) * kRun;
-        float x[kRun][V], k[kRun][V], keep[kRun][V], gy[kRun][V], A[V], S[V], R[V];
-        float before[V];
+    for (int tile = first; tile >= end; --tile, turn ^= 1) {
+        const long t0 = ((long)__builtin_amdgcn_readfirstlane(tile) * s.waves + w) * kRun;
+        const int n = steps_before(t0, len), n_all = steps_before(t0, steps);
+        const bool full = n == kRun && whole;
+        Vec<T, V> x[kRun], gy[kRun];
+        float m[kRun][V], before[V];  // m: 1 - a, or -a where that is less: the smaller of the two has its full precision
+        float A[V], S[V], R[V];       // product of the a, state behind these steps, a u of the first of them, from zero
 #pragma unroll
         for (int i = 0; i < V; ++i)
-            before[i] = c + i < a.channels ? a.checkpoints[(tile * a.batch + b) * a.channels + c + i] : 0.0f;
-        if (len > 0) {
-            Vec<T, V> xv[kRun], gv[kRun], yv[kRun];
-#pragma unroll
-            for (int t = 0; t < kRun; ++t) {
-                const long at = t0 + t < len ? t0 + t : len - 1;
-                xv[t] = xr.load(at);
-                gv[t] = gr.load(at);
-                yv[t] = yr.load(at);
+            before[i] = c + i < a.channels ? a.checkpoints[((long)tile * a.batch + b) * a.channels + c + i] : 0.0f;
+        auto read = [&](auto all) {
+            constexpr bool FULL = decltype(all)::value;
+            Vec<T, V> gate[kRun];
+            xr.template load<FULL>(x, t0, n, len, c, a.channels);
+            gr.template load<FULL>(gate, t0, n, len, c, a.channels);
+            yr.template load<FULL>(gy, t0, n, len, c, a.channels);
+            if (!FULL && n < kRun) {
+                cut_run<T, V>(x, n);
+                cut_run<T, V>(gy, n);
             }
 #pragma unroll
-            for (int t = 0; t < kRun; ++t) {
-                const bool live = t0 + t < len;
+            for (int i = 0; i < V; ++i) {
+                A[i] = 1.0f;
+                S[i] = R[i] = 0.0f;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    sigmoid_pair(gr.value(gv[t], i) + bias[i], keep[t][i], k[t][i]);
-                    x[t][i] = live ? xr.value(xv[t], i) : 0.0f;
-                    gy[t][i] = live ? yr.value(yv[t], i) : 0.0f;
-                    k[t][i] = live ? k[t][i] : 0.0f;
-                    keep[t][i] = live ? keep[t][i] : 1.0f;
+                for (int t = 0; t < kRun; ++t) {
+                    float e, k = closed((float)gate[t][i], bias2[i], e);
+                    const bool small = e < 1.0f;
+                    const float ek = e * k;
+                    float keep = small ? ek : 1.0f - k;  // with its own precision: R sums its products
+                    m[t][i] = small ? -ek : k;
+                    if (!FULL && t >= n) {
+                        m[t][i] = k = 0.0f;
+                        keep = 1.0f;
+                    }
+                    A[i] *= keep;
+                    S[i] = fmaf(k, (float)x[t][i] - S[i], S[i]);
+                    R[i] = fmaf(A[i], (float)gy[t][i], R[i]);
                 }
             }
+        };
+        if (full) {
+            read(std::true_type{});
+        } else if (len > 0) {
+            read(std::false_type{});
         } else {
 #pragma unroll
-            for (int t = 0; t < kRun; ++t)
+            for (int t = 0; t < kRun; ++t) {
+                x[t] = gy[t] = Vec<T, V>{};
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    x[t][i] = k[t][i] = gy[t][i] = 0.0f;
-                    keep[t][i] = 1.0f;
-                }
+                for (int i = 0; i < V; ++i) m[t][i] = 0.0f;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                A[i] = 1.0f;
+                S[i] = R[i] = 0.0f;
+            }
         }
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            A[i] = 1.0f, S[i] = R[i] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < kRun; ++t) {
-                A[i] *= keep[t][i];
-                S[i] = fmaf(k[t][i], x[t][i] - S[i], S[i]);
-            }
-#pragma unroll
-            for (int t = kRun - 1; t >= 0; --t) R[i] = keep[t][i] * (gy[t][i] + R[i]);
             sA[turn][w][lane * V + i] = A[i];
             sS[turn][w][lane * V + i] = S[i];
             sR[turn][w][lane * V + i] = R[i];
@@ -374,15 +487,20 @@ __global__ __launch_bounds__(kLanes *kWaves) void recurrence_backward_kernel(Rec
                 if (tile > 0) announce_run<V>(ch, s, tile, col, lane, At, Rt);
                 look_back<V>(ch, s, tile, col, 1, lane, carry);
             }
+            float after[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) after[i] = fmaf(At[i], carry[i], Rt[i]);
+            if (s.chain && tile > 0) announce_state<V>(ch, s, tile, col, lane, after);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 carried[lane * V + i] = carry[i];
-                carry[i] = fmaf(At[i], carry[i], Rt[i]);
+                carry[i] = after[i];
             }
-            if (s.chain && tile > 0) announce_state<V>(ch, s, tile, col, lane, carry);
         }
         __syncthreads();
         float g[V], sum[V], h[kRun][V];  // h: the state before each step
+#pragma unroll
+        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]), forget<T, V>(gy[t]);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             g[i] = carried[lane * V + i];
@@ -398,24 +516,37 @@ __global__ __launch_bounds__(kLanes *kWaves) void recurrence_backward_kernel(Rec
         for (int i = 0; i < V; ++i) {
             h[0][i] = before[i];
 #pragma unroll
-            for (int t = 1; t < kRun; ++t) h[t][i] = fmaf(k[t - 1][i], x[t - 1][i] - h[t - 1][i], h[t - 1][i]);
-        }
-#pragma unroll
-        for (int t = kRun - 1; t >= 0; --t) {
-            float gx[V], gz[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float u = gy[t][i] + g[i];
-                gx[i] = k[t][i] * u;
-                gz[i] = gx[i] * (h[t][i] - x[t][i]) * keep[t][i];
-                sum[i] += gz[i];
-                g[i] = keep[t][i] * u;
-            }
-            if (t0 + t < a.steps) {
-                if (a.grad_x.data != nullptr) store_lane<T, V>(a.grad_x, b, t0 + t, c, a.channels, gx);
-                if (a.grad_gate.data != nullptr) store_lane<T, V>(a.grad_gate, b, t0 + t, c, a.channels, gz);
+            for (int t = 1; t < kRun; ++t) {
+                const float k = m[t - 1][i] < 0.0f ? 1.0f + m[t - 1][i] : m[t - 1][i];
+                h[t][i] = fmaf(k, (float)x[t - 1][i] - h[t - 1][i], h[t - 1][i]);
             }
         }
+#pragma unroll
+        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]);
+        auto write = [&](auto all) {
+            constexpr bool FULL = decltype(all)::value;
+            const char *to_x = gxr.row(t0 + kRun - 1), *to_gate = ggr.row(t0 + kRun - 1);
+#pragma unroll
+            for (int t = kRun - 1; t >= 0; --t, to_x -= gxr.st, to_gate -= ggr.st) {
+                float gx[V], gz[V];
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    const bool small = m[t][i] < 0.0f;
+                    const float k = small ? 1.0f + m[t][i] : m[t][i], keep = small ? -m[t][i] : 1.0f - m[t][i];
+                    const float u = (float)gy[t][i] + g[i];
+                    gx[i] = k * u;
+                    g[i] = keep * u;
+                    gz[i] = k * (h[t][i] - (float)x[t][i]) * g[i];
+                    sum[i] += gz[i];
+                }
+                if (FULL || t < n_all) {
+                    if (a.grad_x.data != nullptr) gxr.template store<FULL>(to_x, c, a.channels, gx);
+                    if (a.grad_gate.data != nullptr) ggr.template store<FULL>(to_gate, c, a.channels, gz);
+                }
+            }
+        };
+        if (full) write(std::true_type{});
+        else write(std::false_type{});
         if (a.state_out != nullptr && tile == 0 && w == 0)
 #pragma unroll
             for (int i = 0; i < V; ++i)
@@ -431,7 +562,7 @@ __global__ __launch_bounds__(kLanes *kWaves) void recurrence_backward_kernel(Rec
                 for (int i = 0; i < V; ++i) {
                     float v = 0.0f;
                     for (int j = 0; j < s.waves; ++j) v += sR[turn][j][lane * V + i];
-                    if (c + i < a.channels) partial[(tile * a.batch + b) * a.channels + c + i] = v;
+                    if (c + i < a.channels) partial[((long)tile * a.batch + b) * a.channels + c + i] = v;
                 }
         }
     }
@@ -472,33 +603,35 @@ __global__ __launch_bounds__(256) void recurrence_step_kernel(RecArgs a)
     if (a.state_out != nullptr) store_some<V>(a.state_out + at, h, left);
 }
 
-// grad_bias: the sum of `rows` rows of sums, 16 channels and 16 slices of the rows a workgroup, in a fixed order.
-__global__ __launch_bounds__(256) void recurrence_bias_kernel(const float *partial, long rows, int channels, float factor, float *out)
+// grad_bias: the sum of `rows` rows of sums.
+__global__ __launch_bounds__(kSumThreads) void recurrence_bias_kernel(const float *partial, long rows, int channels, float factor, float *out)
 {
-    __shared__ float part[16][17];
-    const int i = threadIdx.x & 15, slice = threadIdx.x >> 4, at = blockIdx.x * 16 + i;
-    float sum = 0.0f;
-    if (at < channels)
-        for (long r = slice; r < rows; r += 16) sum += partial[r * channels + at];
-    part[slice][i] = sum;
-    __syncthreads();
-    if (slice != 0 || at >= channels) return;
-    for (int k = 1; k < 16; ++k) sum += part[k][i];
-    out[at] = sum * factor;
+    __shared__ float part[kSumSlices][kSumColumns];
+    const int at = blockIdx.x * kSumColumns + threadIdx.x % kSumColumns;
+    const float sum = slices_sum(at < channels ? slice_sum(partial + at, channels, rows, threadIdx.x / kSumColumns) : 0.0f, part);
+    if (threadIdx.x < kSumColumns && at < channels) out[at] = sum * factor;
 }
 
-// V: channels of a lane, 2 where the channels of every tensor lie side by side
-static int lane_channels(const RecArgs &a)
+static hipError_t launch_bias(const float *partial, long rows, const RecArgs &a, hipStream_t s)
 {
-    if (a.channels < 2) return 1;
+    const int blocks = (a.channels + kSumColumns - 1) / kSumColumns;
+    kernel_log_add("recurrence_bias_kernel", (long)blocks * kSumThreads);
+    FBFC_LAUNCH(recurrence_bias_kernel, dim3(blocks), dim3(kSumThreads), 0, s, partial, rows, a.channels, a.factor, a.grad_bias);
+    return hipGetLastError();
+}
+
+// Whether the channels of every tensor lie side by side, in rows that 32 bits reach over.
+static bool dense(int type, const RecArgs &a)
+{
+    if (a.channels < (type == kF32 ? 1 : 2) || a.channels > 1 << 29) return false;
     for (const Steps *t : {&a.x, &a.gate, &a.y, &a.grad_x, &a.grad_gate})
-        if (t->data != nullptr && t->sc != 1) return 1;
-    return 2;
+        if (t->data != nullptr && t->sc != 1) return false;
+    return true;
 }
 
 size_t recurrence_checkpoint_bytes(int batch, int channels, long steps)
 {
-    return (size_t)shape_of(batch, channels, steps, 1).tiles * batch * channels * sizeof(float);
+    return (size_t)shape_of(batch, channels, steps, 1).tiles * (size_t)batch * channels * sizeof(float);
 }
 
 size_t recurrence_workspace_bytes(int batch, int channels, long steps)
@@ -515,8 +648,8 @@ size_t recurrence_workspace_bytes(int batch, int channels, long steps)
 
 bool recurrence_fits(int batch, int channels, long steps)
 {
-    const Shape s = shape_of(batch, channels, steps, 1);
-    return s.tiles < (1L << 31) / s.cols && (long)batch * channels < (1L << 38);
+    const long tiles = (steps + kRun * kWaves - 1) / (kRun * kWaves) + 1, cols = (channels + kLanes - 1L) / kLanes * batch;
+    return cols < 1L << 31 && tiles < (1L << 31) / (cols < 1 ? 1 : cols);
 }
 
 static hipError_t clear_chain(const RecArgs &a, const Shape &s, int v, hipStream_t stream)
@@ -529,11 +662,12 @@ static hipError_t clear_chain(const RecArgs &a, const Shape &s, int v, hipStream
 }
 
 template <typename T>
-static hipError_t forward_typed(const RecArgs &a, hipStream_t stream)
+static hipError_t forward_typed(int type, const RecArgs &a, hipStream_t stream)
 {
-    const int v = lane_channels(a);
+    const bool side = dense(type, a);
+    const int v = side ? kLaneChannels<T, true> : 1;
     if (a.steps <= 1) {
-        const bool wide = v == 2 && a.channels >= 4;
+        const bool wide = side && a.channels >= 4;
         const long lanes = (long)a.batch * ((a.channels + (wide ? 3 : 0)) / (wide ? 4 : 1));
         const dim3 grid((unsigned)((lanes + 255) / 256));
         kernel_log_add("recurrence_step_kernel", (long)grid.x * 256);
@@ -546,17 +680,18 @@ static hipError_t forward_typed(const RecArgs &a, hipStream_t stream)
         const hipError_t e = clear_chain(a, s, v, stream);
         if (e != hipSuccess) return e;
     }
-    const dim3 grid((unsigned)(s.chain ? s.tiles * s.cols : s.cols)), block(s.waves * kLanes);
+    const dim3 grid(s.chain ? s.tiles * s.cols : s.cols), block(s.waves * kLanes);
     kernel_log_add(s.chain ? "recurrence_forward_kernel<chain>" : "recurrence_forward_kernel", (long)grid.x * block.x);
-    if (v == 2) FBFC_LAUNCH((recurrence_forward_kernel<T, 2>), grid, block, 0, stream, a);
-    else FBFC_LAUNCH((recurrence_forward_kernel<T, 1>), grid, block, 0, stream, a);
+    if (side) FBFC_LAUNCH((recurrence_forward_kernel<T, true>), grid, block, 0, stream, a);
+    else FBFC_LAUNCH((recurrence_forward_kernel<T, false>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
 
 template <typename T>
-static hipError_t backward_typed(const RecArgs &a, hipStream_t stream)
+static hipError_t backward_typed(int type, const RecArgs &a, hipStream_t stream)
 {
-    const int v = lane_channels(a);
+    const bool side = dense(type, a);
+    const int v = side ? kLaneChannels<T, true> : 1;
     const Shape s = shape_of(a.batch, a.channels, a.steps, v);
     float *partial = nullptr;
     if (a.grad_bias != nullptr)
@@ -566,21 +701,17 @@ static hipError_t backward_typed(const RecArgs &a, hipStream_t stream)
         const hipError_t e = clear_chain(a, s, v, stream);
         if (e != hipSuccess) return e;
     }
-    const dim3 grid((unsigned)(s.chain ? s.tiles * s.cols : s.cols)), block(s.waves * kLanes);
+    const dim3 grid(s.chain ? s.tiles * s.cols : s.cols), block(s.waves * kLanes);
     kernel_log_add(s.chain ? "recurrence_backward_kernel<chain>" : "recurrence_backward_kernel", (long)grid.x * block.x);
-    if (v == 2) FBFC_LAUNCH((recurrence_backward_kernel<T, 2>), grid, block, 0, stream, a, partial);
-    else FBFC_LAUNCH((recurrence_backward_kernel<T, 1>), grid, block, 0, stream, a, partial);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || partial == nullptr) return e;
-    const int blocks = (a.channels + 15) / 16;
-    kernel_log_add("recurrence_bias_kernel", blocks * 256L);
-    FBFC_LAUNCH(recurrence_bias_kernel, dim3(blocks), dim3(256), 0, stream, partial, s.tiles * a.batch, a.channels, a.factor, a.grad_bias);
-    return hipGetLastError();
+    if (side) FBFC_LAUNCH((recurrence_backward_kernel<T, true>), grid, block, 0, stream, a, partial);
+    else FBFC_LAUNCH((recurrence_backward_kernel<T, false>), grid, block, 0, stream, a, partial);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess || partial == nullptr ? e : launch_bias(partial, (long)s.tiles * a.batch, a, stream);
 }
 
 hipError_t launch_recurrence_forward(int type, const RecArgs &a, hipStream_t s)
 {
-    return type == kF32 ? forward_typed<float>(a, s) : type == kBF16 ? forward_typed<bf16>(a, s) : forward_typed<f16>(a, s);
+    return type == kF32 ? forward_typed<float>(type, a, s) : type == kBF16 ? forward_typed<bf16>(type, a, s) : forward_typed<f16>(type, a, s);
 }
 
 hipError_t launch_recurrence_backward(int type, const RecArgs &a, hipStream_t s)
@@ -594,12 +725,9 @@ hipError_t launch_recurrence_backward(int type, const RecArgs &a, hipStream_t s)
             const hipError_t e = launch_recurrence_forward(type, step, s);
             if (e != hipSuccess) return e;
         }
-        if (a.grad_bias == nullptr) return hipSuccess;
-        kernel_log_add("recurrence_bias_kernel", (a.channels + 15) / 16 * 256L);
-        FBFC_LAUNCH(recurrence_bias_kernel, dim3((a.channels + 15) / 16), dim3(256), 0, s, nullptr, 0L, a.channels, a.factor, a.grad_bias);
-        return hipGetLastError();
+        return a.grad_bias == nullptr ? hipSuccess : launch_bias(nullptr, 0, a, s);
     }
-    return type == kF32 ? backward_typed<float>(a, s) : type == kBF16 ? backward_typed<bf16>(a, s) : backward_typed<f16>(a, s);
+    return type == kF32 ? backward_typed<float>(type, a, s) : type == kBF16 ? backward_typed<bf16>(type, a, s) : backward_typed<f16>(type, a, s);
 }
 
 }  // namespace fbfc

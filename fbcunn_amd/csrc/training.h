@@ -14,11 +14,14 @@ struct AdamwPiece {
     long first;
     long n;
 };
-constexpr int kAdamwPiece = 4096;   // parameters of a piece
+// Parameters of a piece: enough for a workgroup to hold all its loads in flight, or, where that leaves CUs
+// without a piece (below 2048 pieces), as few as one load each.
+constexpr int kAdamwPiece = 4096, kAdamwSmallPiece = 1024;
 constexpr int kAdamwBlock = 256;    // 8-bit states: values that share a scale
 // What a step takes from the number of steps before it; on the device, brought up to date by the last workgroup.
 struct AdamwClock {
     long t;             // steps taken
+    double power1, power2;  // beta1^(t + 1), beta2^(t + 1)
     double inv_bias1;   // 1 / (1 - beta1^(t + 1))
     float inv_root2;    // 1 / sqrt(1 - beta2^(t + 1))
     unsigned key;       // of the random numbers of step t + 1

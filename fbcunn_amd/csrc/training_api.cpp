@@ -94,7 +94,7 @@ static int adamw_check(const fbfc_adamw_config *c, const fbfc_adamw_tensor *tens
         if (t.n > 0 && (t.param == nullptr || t.grad == nullptr)) return fail(FBFC_ERR_INVALID_ARGUMENT, "null tensor");
         if (!aligned(t.param, pb) || !aligned(t.grad, gb))
             return fail(FBFC_ERR_INVALID_ARGUMENT, "tensors must be aligned to their type");
-        pieces += (t.n + fbfc::kAdamwPiece - 1) / fbfc::kAdamwPiece;
+        pieces += (t.n + fbfc::kAdamwSmallPiece - 1) / fbfc::kAdamwSmallPiece;
     }
     if (pieces > INT32_MAX) return fail(FBFC_ERR_UNSUPPORTED_SIZE, "too many parameters for one optimizer");
     const size_t n = (size_t)fbfc_adamw_state_elements(tensors, count);
@@ -125,12 +125,14 @@ static int adamw_create(const fbfc_adamw_config *c, const fbfc_adamw_tensor *ten
     if (rc != FBFC_OK) return rc;
     std::vector<fbfc::AdamwPiece> pieces;
     const size_t pb = type_bytes(c->param_type), gb = type_bytes(c->grad_type);
-    long first = 0;
+    long first = 0, n = 0;
+    for (int i = 0; i < count; ++i) n += tensors[i].n;
+    const long size = n < 2048L * fbfc::kAdamwPiece ? fbfc::kAdamwSmallPiece : fbfc::kAdamwPiece;
     for (int i = 0; i < count; ++i) {
         const fbfc_adamw_tensor &t = tensors[i];
-        for (long o = 0; o < t.n; o += fbfc::kAdamwPiece)
+        for (long o = 0; o < t.n; o += size)
             pieces.push_back({static_cast<char *>(t.param) + o * pb, static_cast<const char *>(t.grad) + o * gb, first + o,
-                              std::min<long>(t.n - o, fbfc::kAdamwPiece)});
+                              std::min(t.n - o, size)});
         first += (t.n + fbfc::kAdamwBlock - 1) / fbfc::kAdamwBlock * fbfc::kAdamwBlock;
     }
     fbfc_adamw *p = new (std::nothrow) fbfc_adamw();
