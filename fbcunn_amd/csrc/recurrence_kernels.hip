@@ -28,9 +28,13 @@
 
 namespace fbfc {
 
-constexpr int kRun = 16;      // steps of a wavefront
+constexpr int kRun = 16;     // steps of a wavefront
 constexpr int kWaves = 8;     // wavefronts of a workgroup, at most
 constexpr int kLanes = 64;
+// Workgroups that the GPU holds, two on each CU: as many columns or more are walked over by one workgroup each, fewer by
+// several, which hand the state from tile to tile.
+constexpr int kGroups = 512;
+constexpr int kHead = 256;    // bytes of the workspace before the announcements
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Announcements.  A word is announced once it differs from what the workspace is filled with, all ones (a NaN that
@@ -63,8 +67,7 @@ __host__ __device__ __forceinline__ Shape shape_of(int batch, int channels, long
     s.blocks = (channels + kLanes * v - 1) / (kLanes * v);
     s.tiles = (int)((runs + s.waves - 1) / s.waves);  // recurrence_fits(): tiles * cols is below 2^31
     s.cols = batch * s.blocks;
-    // 512 workgroups fill the GPU by themselves; fewer leave CUs idle, and their tiles are then spread
-    s.chain = s.tiles > 1 && s.cols < 512;
+    s.chain = s.tiles > 1 && s.cols < kGroups;
     return s;
 }
 
@@ -72,44 +75,80 @@ __device__ __forceinline__ Chain chain_of(unsigned char *workspace, const Shape 
 {
     Chain c;
     c.ticket = reinterpret_cast<unsigned *>(workspace);
-    c.runs = reinterpret_cast<word64 *>(workspace + 256);
+    c.runs = reinterpret_cast<word64 *>(workspace + kHead);
     c.states = reinterpret_cast<unsigned *>(c.runs + (long)s.tiles * s.cols * kLanes * v);
     return c;
 }
-static size_t chain_bytes(const Shape &s, int v) { return 256 + (size_t)s.tiles * s.cols * kLanes * v * 12; }
+static size_t chain_bytes(const Shape &s, int v) { return kHead + (size_t)s.tiles * s.cols * kLanes * v * 12; }
 
 __global__ __launch_bounds__(256) void recurrence_clear_kernel(uint4 *p, long n)
 {
     for (long i = blockIdx.x * 256L + threadIdx.x; i < n; i += gridDim.x * 256L) p[i] = uint4{kUnset, kUnset, kUnset, kUnset};
 }
 
-// The state in front of tile `at` of column `col`, of this lane's channels; `dir` is where the tile before it lies.
+template <int V>
+__device__ __forceinline__ void fold(float (&h)[V], const word64 (&run)[V])
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) h[i] = fmaf(__uint_as_float((unsigned)run[i]), h[i], __uint_as_float((unsigned)(run[i] >> 32)));
+}
+
+// The state in front of tile `at` of column `col`, of this lane's channels; `dir` is where the tile before it lies.  Four
+// tiles are asked at once: what a tile announces takes a microsecond to reach another compute unit, and one at a
+// time the walk back would never catch up.
+constexpr int kAsk = 4;
 template <int V>
 __device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, int at, int col, int dir, int lane, float (&h)[V])
 {
-    const int cell = kLanes * V;
-    int j = at + dir;
+    const long cell = (long)kLanes * V, place = (long)col * cell + lane * V, row = (long)s.cols * cell;
+    int j = at + dir;  // the nearest of the tiles that are asked
     while (true) {
-        bool state = true, run = true;
+        unsigned state[kAsk][V];
+        word64 run[kAsk][V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const long k = (long)(j * s.cols + col) * cell + lane * V + i;
-            const unsigned p = __hip_atomic_load(ch.states + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            const word64 r = __hip_atomic_load(ch.runs + k, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            h[i] = __uint_as_float(p);
-            state &= p != kUnset;
-            run &= r != kUnset2;
+        for (int q = 0; q < kAsk; ++q) {
+            int k = j + dir * q;
+            k = k < 0 ? 0 : k < s.tiles ? k : s.tiles - 1;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                state[q][i] = __hip_atomic_load(ch.states + k * row + place + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                run[q][i] = __hip_atomic_load(ch.runs + k * row + place + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            }
         }
-        if (__all(state)) break;
-        if (__all(run)) j += dir;  // the first tile announces no run, so the search ends there
+        int hit = -1, known = 0;  // the tile whose state is announced; how many before it have announced their runs
+#pragma unroll
+        for (int q = 0; q < kAsk; ++q) {
+            bool has_state = true, has_run = true;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                has_state &= state[q][i] != kUnset;
+                has_run &= run[q][i] != kUnset2;
+            }
+            if (hit < 0 && known == q) {
+                if (__all(has_state)) {
+                    hit = q;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) h[i] = __uint_as_float(state[q][i]);
+                } else if (__all(has_run)) {
+                    ++known;  // never the first tile, which announces no run: the walk ends there
+                }
+            }
+        }
+        if (hit >= 0) {
+#pragma unroll
+            for (int q = kAsk - 1; q >= 0; --q)
+                if (q < hit) fold<V>(h, run[q]);
+            break;
+        }
+        if (known == kAsk) j += dir * kAsk;
         else __builtin_amdgcn_s_sleep(1);
     }
+    // the tiles that earlier rounds passed over
     for (j -= dir; j != at; j -= dir) {
+        word64 run[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            const word64 r = __hip_atomic_load(ch.runs + (long)(j * s.cols + col) * cell + lane * V + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-            h[i] = fmaf(__uint_as_float((unsigned)r), h[i], __uint_as_float((unsigned)(r >> 32)));
-        }
+        for (int i = 0; i < V; ++i) run[i] = __hip_atomic_load(ch.runs + j * row + place + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        fold<V>(h, run);
     }
 }
 
@@ -213,32 +252,19 @@ __device__ __forceinline__ float closed(float gate, float bias2, float &e)
     return __builtin_amdgcn_rcpf(1.0f + e);
 }
 
-// Where a workgroup works: its column (sequence and block of channels) and the tiles it walks over.
-struct Place {
-    int col, order;     // order: which of the column's tiles, counted in the order in which they depend on each other
-    int b, c;
-    long len;           // steps of the sequence
-};
-template <int V>
-__device__ __forceinline__ Place place_of(const int *lengths, long steps, const Shape &s, const Chain &ch, unsigned *given)
+// Tickets count the tiles of all columns (sequences and blocks of channels) in the order in which they depend on each
+// other, those of different columns side by side: what is worked on at one time lies in the same rows of memory.  Other ways
+// of giving out tiles, on the forward pass over 131072 steps of 2048 channels in bf16 (388 us so): a counter for each column, 399
+// us; that with the columns kept to one XCD, 454 us; workgroups that stay and draw their next tile ahead, 417 us.
+__device__ __forceinline__ unsigned draw(const Chain &ch)
 {
-    unsigned work = blockIdx.x;
-    if (s.chain) {
-        if (threadIdx.x == 0) *given = __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
-        __syncthreads();
-        work = __builtin_amdgcn_readfirstlane(*given);
-    }
-    Place p;
-    p.order = __builtin_amdgcn_readfirstlane(work / (unsigned)s.cols);
-    p.col = __builtin_amdgcn_readfirstlane(work % (unsigned)s.cols);
-    p.b = p.col / s.blocks;
-    p.c = p.col % s.blocks * kLanes * V + (threadIdx.x & 63) * V;
-    p.len = steps;
-    if (lengths != nullptr) {
-        const long n = __builtin_amdgcn_readfirstlane(lengths[p.b]);
-        p.len = n < 0 ? 0 : n < p.len ? n : p.len;
-    }
-    return p;
+    return __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+}
+__device__ __forceinline__ long length_of(const int *lengths, int b, long steps)
+{
+    if (lengths == nullptr) return steps;
+    const long n = __builtin_amdgcn_readfirstlane(lengths[b]);
+    return n < 0 ? 0 : n < steps ? n : steps;
 }
 
 // How many of the 16 steps from t0 on lie before `end`.
@@ -253,6 +279,43 @@ __device__ __forceinline__ void cut_run(Vec<T, V> (&v)[kRun], int n)
         if (t >= n) v[t] = Vec<T, V>{};
 }
 
+// The runs of wavefronts 0 to count - 1, as one; and of wavefronts from to kWaves - 1, the last of them first.  Those that
+// the workgroup does not have hold identities, so that every read has a fixed place and none waits for another.
+template <int V>
+__device__ __forceinline__ void join(float (&A)[V], float (&S)[V], const float (*a)[kLanes * V], const float (*s)[kLanes * V], int count, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = 1.0f, S[i] = 0.0f;
+#pragma unroll
+    for (int j = 0; j < kWaves; ++j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float Aj = a[j][lane * V + i], Sj = s[j][lane * V + i];
+            A[i] = j < count ? A[i] * Aj : A[i];
+            S[i] = j < count ? fmaf(Aj, S[i], Sj) : S[i];
+        }
+}
+template <int V>
+__device__ __forceinline__ void join_back(float (&A)[V], float (&R)[V], const float (*a)[kLanes * V], const float (*r)[kLanes * V], int from, int lane)
+{
+#pragma unroll
+    for (int i = 0; i < V; ++i) A[i] = 1.0f, R[i] = 0.0f;
+#pragma unroll
+    for (int j = kWaves - 1; j >= 0; --j)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float Aj = a[j][lane * V + i], Rj = r[j][lane * V + i];
+            A[i] = j >= from ? A[i] * Aj : A[i];
+            R[i] = j >= from ? fmaf(Aj, R[i], Rj) : R[i];
+        }
+}
+template <int V>
+__device__ __forceinline__ void fill_runs(float (*to)[kWaves][kLanes * V], int waves, float v)
+{
+    for (int j = waves; j < kWaves; ++j)
+        for (int i = threadIdx.x; i < kLanes * V; i += blockDim.x) to[0][j][i] = to[1][j][i] = v;
+}
+
 template <typename T, bool DENSE>
 __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(RecArgs a)
 {
@@ -263,82 +326,75 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
     const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    const Place p = place_of<V>(a.lengths, steps, s, ch, &given);
-    const long len = p.len;
-    const int col = p.col, end = s.chain ? p.order + 1 : s.tiles, b = p.b, c = p.c;
-    const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
-    float bias2[V], carry[V];  // carry: wavefront 0, the state before the tile
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias2[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] * kLog2e : 0.0f;
-        carry[i] = a.state_in != nullptr && c + i < a.channels ? a.state_in[(long)b * a.channels + c + i] : 0.0f;
+    unsigned ticket = blockIdx.x;
+    const unsigned all = (unsigned)s.tiles * s.cols;
+    if (s.chain) {
+        if (threadIdx.x == 0) given = draw(ch);
+        __syncthreads();
+        ticket = __builtin_amdgcn_readfirstlane(given);
     }
-    const bool whole = __all(c + V <= a.channels);
-    int turn = 0;
-    for (int tile = p.order; tile < end; ++tile, turn ^= 1) {
+    fill_runs<V>(sA, s.waves, 1.0f);
+    fill_runs<V>(sS, s.waves, 0.0f);
+    float carry[V];  // in the first wavefront: the state before the tile
+    for (int turn = 0; ticket < all; turn ^= 1, ticket = s.chain ? all : ticket + s.cols) {
+        const int order = ticket / (unsigned)s.cols, col = ticket % (unsigned)s.cols, tile = order;
+        const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
+        const long len = length_of(a.lengths, b, steps);
+        const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
+        const bool whole = __all(c + V <= a.channels);
+        float bias2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            bias2[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] * kLog2e : 0.0f;
+            if (order == 0) carry[i] = a.state_in != nullptr && c + i < a.channels ? a.state_in[(long)b * a.channels + c + i] : 0.0f;
+        }
         const long t0 = ((long)__builtin_amdgcn_readfirstlane(tile) * s.waves + w) * kRun;
         const int n = steps_before(t0, len), n_all = steps_before(t0, steps);
         const bool full = n == kRun && whole;
-        Vec<T, V> x[kRun];
-        float k[kRun][V], A[V], S[V];  // k: 1 - a
+        // The gates are evaluated twice: kept, they would take as many registers again, and half the wavefronts would fit.
+        Vec<T, V> x[kRun], gate[kRun];
+        float A[V], S[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            A[i] = 1.0f;
+            S[i] = 0.0f;
+        }
         auto read = [&](auto all) {
             constexpr bool FULL = decltype(all)::value;
-            Vec<T, V> gate[kRun];
             xr.template load<FULL>(x, t0, n, len, c, a.channels);
             gr.template load<FULL>(gate, t0, n, len, c, a.channels);
             if (!FULL && n < kRun) cut_run<T, V>(x, n);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                A[i] = 1.0f;
-                S[i] = 0.0f;
+            for (int t = 0; t < kRun; ++t) {
 #pragma unroll
-                for (int t = 0; t < kRun; ++t) {
-                    float e;
-                    k[t][i] = closed((float)gate[t][i], bias2[i], e);
-                    if (!FULL && t >= n) k[t][i] = 0.0f;
-                    A[i] = fmaf(-k[t][i], A[i], A[i]);
-                    S[i] = fmaf(k[t][i], (float)x[t][i] - S[i], S[i]);
+                for (int i = 0; i < V; ++i) {
+                    float e, k = closed((float)gate[t][i], bias2[i], e);
+                    if (!FULL && t >= n) k = 0.0f;
+                    A[i] = fmaf(-k, A[i], A[i]);
+                    S[i] = fmaf(k, (float)x[t][i] - S[i], S[i]);
                 }
+                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         };
-        if (full) {
-            read(std::true_type{});
-        } else if (len > 0) {
-            read(std::false_type{});
-        } else {
-#pragma unroll
-            for (int t = 0; t < kRun; ++t) {
-                x[t] = Vec<T, V>{};
-#pragma unroll
-                for (int i = 0; i < V; ++i) k[t][i] = 0.0f;
-            }
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                A[i] = 1.0f;
-                S[i] = 0.0f;
-            }
-        }
+        if (full) read(std::true_type{});
+        else if (len > 0) read(std::false_type{});
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             sA[turn][w][lane * V + i] = A[i];
             sS[turn][w][lane * V + i] = S[i];
         }
         __syncthreads();
+        // the runs of the wavefronts before this one, as one; of the whole tile in the first wavefront
+        float Ap[V], Sp[V];
+        join<V>(Ap, Sp, sA[turn], sS[turn], w == 0 ? kWaves : w, lane);
         if (w == 0) {
-            for (int j = 1; j < s.waves; ++j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float Aj = sA[turn][j][lane * V + i];
-                    A[i] *= Aj;
-                    S[i] = fmaf(Aj, S[i], sS[turn][j][lane * V + i]);
-                }
             if (s.chain && tile > 0) {
-                if (tile + 1 < s.tiles) announce_run<V>(ch, s, tile, col, lane, A, S);
+                if (tile + 1 < s.tiles) announce_run<V>(ch, s, tile, col, lane, Ap, Sp);
                 look_back<V>(ch, s, tile, col, -1, lane, carry);
             }
             float after[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) after[i] = fmaf(A[i], carry[i], S[i]);
+            for (int i = 0; i < V; ++i) after[i] = fmaf(Ap[i], carry[i], Sp[i]);
             if (s.chain && tile + 1 < s.tiles) announce_state<V>(ch, s, tile, col, lane, after);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -346,17 +402,16 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
                 if (a.checkpoints != nullptr && c + i < a.channels)
                     a.checkpoints[((long)tile * a.batch + b) * a.channels + c + i] = carry[i];
                 carry[i] = after[i];
+                Ap[i] = 1.0f;
+                Sp[i] = 0.0f;
             }
         }
         __syncthreads();
         float h[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) h[i] = carried[lane * V + i];
-        for (int j = 0; j < w; ++j)
+        for (int i = 0; i < V; ++i) h[i] = fmaf(Ap[i], carried[lane * V + i], Sp[i]);
 #pragma unroll
-            for (int i = 0; i < V; ++i) h[i] = fmaf(sA[turn][j][lane * V + i], h[i], sS[turn][j][lane * V + i]);
-#pragma unroll
-        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]);
+        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]), forget<T, V>(gate[t]);
         auto write = [&](auto all) {
             constexpr bool FULL = decltype(all)::value;
             const char *to = yr.row(t0);
@@ -365,10 +420,12 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
                 float out[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    h[i] = fmaf(k[t][i], (float)x[t][i] - h[i], h[i]);
+                    float e;
+                    if (FULL || t < n) h[i] = fmaf(closed((float)gate[t][i], bias2[i], e), (float)x[t][i] - h[i], h[i]);
                     out[i] = FULL || t < n ? h[i] : 0.0f;
                 }
                 if (FULL || t < n_all) yr.template store<FULL>(to, c, a.channels, out);
+                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
             }
         };
         if (full) write(std::true_type{});
@@ -381,7 +438,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
 }
 
 template <typename T, bool DENSE>
-__global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(RecArgs a, float *partial)
+__global__ __launch_bounds__(kLanes *kWaves, 2) void recurrence_backward_kernel(RecArgs a, float *partial)
 {
     constexpr int V = kLaneChannels<T, DENSE>;
     __shared__ float sA[2][kWaves][kLanes * V], sS[2][kWaves][kLanes * V], sR[2][kWaves][kLanes * V], carried[kLanes * V];
@@ -390,20 +447,30 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
     const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    const Place p = place_of<V>(a.lengths, steps, s, ch, &given);
-    const long len = p.len;
-    const int col = p.col, first = s.tiles - 1 - p.order, end = s.chain ? first : 0, b = p.b, c = p.c;
-    const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
-        gxr(a.grad_x, b, c, a.channels), ggr(a.grad_gate, b, c, a.channels);
-    float bias2[V], carry[V];  // carry: wavefront 0, a_{t+1} u_{t+1} behind the tile
-#pragma unroll
-    for (int i = 0; i < V; ++i) {
-        bias2[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] * kLog2e : 0.0f;
-        carry[i] = a.state_in != nullptr && c + i < a.channels ? a.state_in[(long)b * a.channels + c + i] : 0.0f;
+    unsigned ticket = blockIdx.x;
+    const unsigned all = (unsigned)s.tiles * s.cols;
+    if (s.chain) {
+        if (threadIdx.x == 0) given = draw(ch);
+        __syncthreads();
+        ticket = __builtin_amdgcn_readfirstlane(given);
     }
-    const bool whole = __all(c + V <= a.channels);
-    int turn = 0;
-    for (int tile = first; tile >= end; --tile, turn ^= 1) {
+    fill_runs<V>(sA, s.waves, 1.0f);
+    fill_runs<V>(sS, s.waves, 0.0f);
+    fill_runs<V>(sR, s.waves, 0.0f);
+    float carry[V];  // in the first wavefront: a_{t+1} u_{t+1} behind the tile
+    for (int turn = 0; ticket < all; turn ^= 1, ticket = s.chain ? all : ticket + s.cols) {
+        const int order = ticket / (unsigned)s.cols, col = ticket % (unsigned)s.cols, tile = s.tiles - 1 - order;
+        const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
+        const long len = length_of(a.lengths, b, steps);
+        const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
+            gxr(a.grad_x, b, c, a.channels), ggr(a.grad_gate, b, c, a.channels);
+        const bool whole = __all(c + V <= a.channels);
+        float bias2[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            bias2[i] = a.bias != nullptr && c + i < a.channels ? a.bias[c + i] * kLog2e : 0.0f;
+            if (order == 0) carry[i] = a.state_in != nullptr && c + i < a.channels ? a.state_in[(long)b * a.channels + c + i] : 0.0f;
+        }
         const long t0 = ((long)__builtin_amdgcn_readfirstlane(tile) * s.waves + w) * kRun;
         const int n = steps_before(t0, len), n_all = steps_before(t0, steps);
         const bool full = n == kRun && whole;
@@ -427,8 +494,11 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
             for (int i = 0; i < V; ++i) {
                 A[i] = 1.0f;
                 S[i] = R[i] = 0.0f;
+            }
 #pragma unroll
-                for (int t = 0; t < kRun; ++t) {
+            for (int t = 0; t < kRun; ++t) {
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
                     float e, k = closed((float)gate[t][i], bias2[i], e);
                     const bool small = e < 1.0f;
                     const float ek = e * k;
@@ -442,6 +512,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
                     S[i] = fmaf(k, (float)x[t][i] - S[i], S[i]);
                     R[i] = fmaf(A[i], (float)gy[t][i], R[i]);
                 }
+                if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few steps at a time, or their parts fill the registers
             }
         };
         if (full) {
@@ -468,61 +539,51 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
             sR[turn][w][lane * V + i] = R[i];
         }
         __syncthreads();
-        if (w == 0) {
-            // the whole tile, from its last wavefront to its first
-            float At[V], Rt[V];
+        // The runs of the wavefronts behind this one, as one; of the whole tile in the first wavefront, which announces them.
+        float Aq[V], Rq[V];
+        join_back<V>(Aq, Rq, sA[turn], sR[turn], w == 0 ? 0 : w + 1, lane);
+        if (w == 0 && s.chain && tile > 0 && tile + 1 < s.tiles) announce_run<V>(ch, s, tile, col, lane, Aq, Rq);
+        // the states inside this wavefront's steps, from the one before the tile
+        {
+            float Ap[V], Sp[V];
+            join<V>(Ap, Sp, sA[turn], sS[turn], w, lane);
+#pragma unroll
+            for (int i = 0; i < V; ++i) before[i] = fmaf(Ap[i], before[i], Sp[i]);
+        }
+        float d[kRun][V];  // the state before each step, less x
+#pragma unroll
+        for (int t = 0; t < kRun; ++t) {
+            forget<T, V>(x[t]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                At[i] = sA[turn][s.waves - 1][lane * V + i];
-                Rt[i] = sR[turn][s.waves - 1][lane * V + i];
+                const float k = m[t][i] < 0.0f ? 1.0f + m[t][i] : m[t][i];
+                d[t][i] = before[i] - (float)x[t][i];
+                before[i] = fmaf(-k, d[t][i], before[i]);
             }
-            for (int j = s.waves - 2; j >= 0; --j)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float Aj = sA[turn][j][lane * V + i];
-                    At[i] *= Aj;
-                    Rt[i] = fmaf(Aj, Rt[i], sR[turn][j][lane * V + i]);
-                }
-            if (s.chain && tile + 1 < s.tiles) {
-                if (tile > 0) announce_run<V>(ch, s, tile, col, lane, At, Rt);
-                look_back<V>(ch, s, tile, col, 1, lane, carry);
-            }
+            if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+        }
+        if (w == 0) {
+            if (s.chain && tile + 1 < s.tiles) look_back<V>(ch, s, tile, col, 1, lane, carry);
             float after[V];
 #pragma unroll
-            for (int i = 0; i < V; ++i) after[i] = fmaf(At[i], carry[i], Rt[i]);
+            for (int i = 0; i < V; ++i) after[i] = fmaf(Aq[i], carry[i], Rq[i]);
             if (s.chain && tile > 0) announce_state<V>(ch, s, tile, col, lane, after);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
                 carried[lane * V + i] = carry[i];
                 carry[i] = after[i];
             }
+            join_back<V>(Aq, Rq, sA[turn], sR[turn], 1, lane);
         }
         __syncthreads();
-        float g[V], sum[V], h[kRun][V];  // h: the state before each step
-#pragma unroll
-        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]), forget<T, V>(gy[t]);
+        float g[V], sum[V];
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            g[i] = carried[lane * V + i];
+            g[i] = fmaf(Aq[i], carried[lane * V + i], Rq[i]);
             sum[i] = 0.0f;
         }
-        for (int j = s.waves - 1; j > w; --j)
 #pragma unroll
-            for (int i = 0; i < V; ++i) g[i] = fmaf(sA[turn][j][lane * V + i], g[i], sR[turn][j][lane * V + i]);
-        for (int j = 0; j < w; ++j)
-#pragma unroll
-            for (int i = 0; i < V; ++i) before[i] = fmaf(sA[turn][j][lane * V + i], before[i], sS[turn][j][lane * V + i]);
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            h[0][i] = before[i];
-#pragma unroll
-            for (int t = 1; t < kRun; ++t) {
-                const float k = m[t - 1][i] < 0.0f ? 1.0f + m[t - 1][i] : m[t - 1][i];
-                h[t][i] = fmaf(k, (float)x[t - 1][i] - h[t - 1][i], h[t - 1][i]);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]);
+        for (int t = 0; t < kRun; ++t) forget<T, V>(gy[t]);
         auto write = [&](auto all) {
             constexpr bool FULL = decltype(all)::value;
             const char *to_x = gxr.row(t0 + kRun - 1), *to_gate = ggr.row(t0 + kRun - 1);
@@ -536,13 +597,14 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
                     const float u = (float)gy[t][i] + g[i];
                     gx[i] = k * u;
                     g[i] = keep * u;
-                    gz[i] = k * (h[t][i] - (float)x[t][i]) * g[i];
+                    gz[i] = k * d[t][i] * g[i];
                     sum[i] += gz[i];
                 }
                 if (FULL || t < n_all) {
                     if (a.grad_x.data != nullptr) gxr.template store<FULL>(to_x, c, a.channels, gx);
                     if (a.grad_gate.data != nullptr) ggr.template store<FULL>(to_gate, c, a.channels, gz);
                 }
+                if (t % 4 == 0) __builtin_amdgcn_sched_barrier(0);
             }
         };
         if (full) write(std::true_type{});

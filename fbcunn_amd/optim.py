@@ -73,6 +73,9 @@ class AdamW:
 
     def step(self, scale=1.0):
         """One step with the gradients times `scale`, on the current stream."""
+        if torch.cuda.current_device() == self.device.index:
+            check(lib().fbfc_adamw_step(self._handle, self.lr, self.weightDecay, scale, _stream()))
+            return
         with torch.cuda.device(self.device):
             check(lib().fbfc_adamw_step(self._handle, self.lr, self.weightDecay, scale, _stream()))
 

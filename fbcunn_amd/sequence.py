@@ -6,7 +6,7 @@ import torch
 
 from . import _lib
 from ._lib import RecurrenceDesc, ResidualNormDesc, Rows, Steps, check, lib
-from .tensors import TYPES, Workspace, _ptr, _stream
+from .tensors import TYPES, Workspace, _ptr, _stream, check_current, signature
 
 __all__ = ["GatedLinearRecurrence", "GatedResidualNorm"]
 
@@ -16,13 +16,13 @@ def _check_activation(t, name, like=None):
         raise TypeError("%s: CUDA support only!" % name)
     if t.dtype not in TYPES:
         raise TypeError("%s must be float32, bfloat16 or float16" % name)
-    if t.device.index != torch.cuda.current_device():
-        raise ValueError("%s is not on the current device" % name)
     if like is not None:
         if t.dtype != like.dtype:
             raise TypeError("%s must be %s" % (name, like.dtype))
         if t.shape != like.shape:
             raise ValueError("%s has the wrong shape" % name)
+        if t.device != like.device:
+            raise ValueError("%s is on another device" % name)
 
 
 def _like(old, t):
@@ -32,8 +32,25 @@ def _like(old, t):
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
-def _steps(t):
-    return None if t is None else ctypes.byref(Steps(t.data_ptr(), *t.stride()))
+class _RecurrenceCall:
+    """What calls of the recurrence on inputs of one signature share: checked sizes and descriptors."""
+
+    def __init__(self, x, gate, channels, dims):
+        _check_activation(x, "x")
+        _check_activation(gate, "gate", x)
+        if x.dim() != dims or x.size(-1) != channels:
+            raise ValueError("x must be (%s%d)" % ("batch, steps, " if dims == 3 else "batch, ", channels))
+        self.shape, self.dtype, self.device, self.index = x.shape, x.dtype, x.device, x.device.index
+        self.batch, steps = x.size(0), x.size(1) if dims == 3 else 1
+        desc = RecurrenceDesc(self.batch, channels, steps, TYPES[x.dtype])
+        self.desc = ctypes.byref(desc)
+        self.checkpointBytes = lib().fbfc_recurrence_checkpoint_bytes(self.desc)
+        self.workspaceBytes = lib().fbfc_recurrence_workspace_bytes(self.desc)
+        whole = (steps * channels, channels, 1)
+        strides = [t.stride() if dims == 3 else (t.stride(0), 0, t.stride(1)) for t in (x, gate)]
+        # x, gate, output, gradients of x and gate, gradient of the output (its strides are those of each call)
+        self.steps = [Steps(0, *s) for s in (strides[0], strides[1], whole, whole, whole, whole)]
+        self.refs = [ctypes.byref(s) for s in self.steps]
 
 
 class GatedLinearRecurrence:
@@ -44,7 +61,8 @@ class GatedLinearRecurrence:
     `state`: the state before the first step, zeros where it is None.  `lengths`: an int32 CUDA tensor with the steps of each
     sequence; behind them nothing is read, and outputs and gradients are zero.  backward (and its halves updateGradInput
     and accGradParameters) follows an updateOutput of the same inputs, from which the module keeps the state before every
-    128 steps; after evaluate() it keeps none and cannot go backward.  step advances sequences by one token."""
+    128 steps; after evaluate() it keeps none and cannot go backward.  step advances sequences by one token.  As in the
+    other modules the outputs are the module's own tensors, which its next call on inputs of the same shape writes again."""
 
     def __init__(self, nChannels, device="cuda"):
         if not isinstance(nChannels, int) or nChannels < 1:
@@ -56,6 +74,7 @@ class GatedLinearRecurrence:
         self.train = True
         self.output = self.state = self.gradInput = self.gradState = None
         self._workspace, self._checkpoints = Workspace(), Workspace()
+        self._calls = {2: (None, None), 3: (None, None)}   # the last signature of step and updateOutput, and its call
         self._forward = None   # (shape, type, lengths, checkpoints) of the updateOutput that backward may follow
 
     def training(self):
@@ -70,95 +89,98 @@ class GatedLinearRecurrence:
     def zeroGradParameters(self):
         self.gradBias.zero_()
 
-    def _inputs(self, input):
+    def _call(self, input, dims):
         if len(input) != 2:
             raise ValueError("the input is [x, gate]")
         x, gate = input
-        _check_activation(x, "x")
-        _check_activation(gate, "gate", x)
-        if x.dim() != 3 or x.size(2) != self.nChannels:
-            raise ValueError("x must be (batch, steps, %d)" % self.nChannels)
-        return x, gate, ctypes.byref(RecurrenceDesc(x.size(0), self.nChannels, x.size(1), TYPES[x.dtype]))
+        of = signature(x, gate)
+        last, call = self._calls[dims]
+        if last != of:
+            call = _RecurrenceCall(x, gate, self.nChannels, dims)
+            self._calls[dims] = (of, call)
+        check_current(call.index)
+        call.steps[0].data, call.steps[1].data = x.data_ptr(), gate.data_ptr()
+        return call
 
-    def _check_state(self, t, name, batch):
+    def _check_state(self, t, name, call):
         if t is None:
-            return
+            return None
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise TypeError("%s: CUDA support only!" % name)
         if t.dtype != torch.float32:
             raise TypeError("%s must be float32" % name)
-        if tuple(t.shape) != (batch, self.nChannels) or not t.is_contiguous() or t.device.index != torch.cuda.current_device():
-            raise ValueError("%s must be a contiguous (%d, %d) tensor on the current device" % (name, batch, self.nChannels))
+        if t.shape != (call.batch, self.nChannels) or not t.is_contiguous() or t.device != call.device:
+            raise ValueError("%s must be a contiguous (%d, %d) tensor on the inputs' device" % (name, call.batch, self.nChannels))
+        return t.data_ptr()
 
     @staticmethod
-    def _check_lengths(t, batch):
+    def _check_lengths(t, call):
         if t is None:
-            return
+            return None
         if not isinstance(t, torch.Tensor) or not t.is_cuda:
             raise TypeError("lengths: CUDA support only!")
         if t.dtype != torch.int32:
             raise TypeError("lengths must be int32")
-        if tuple(t.shape) != (batch,) or not t.is_contiguous() or t.device.index != torch.cuda.current_device():
-            raise ValueError("lengths must be %d contiguous numbers on the current device" % batch)
+        if t.shape != (call.batch,) or not t.is_contiguous() or t.device != call.device:
+            raise ValueError("lengths must be %d contiguous numbers on the inputs' device" % call.batch)
+        return t.data_ptr()
+
+    def _state_like(self, old, call):
+        if old is not None and old.size(0) == call.batch and old.device == call.device:
+            return old
+        return torch.empty(call.batch, self.nChannels, device=call.device)
 
     def updateOutput(self, input, state=None, lengths=None):
-        x, gate, desc = self._inputs(input)
-        batch = x.size(0)
-        self._check_state(state, "state", batch)
-        self._check_lengths(lengths, batch)
-        self.output = _like(self.output, x)
-        if self.state is None or self.state.size(0) != batch or self.state.device != x.device:
-            self.state = torch.empty(batch, self.nChannels, device=x.device)
-        kept = None
-        if self.train:
-            kept = self._checkpoints.take(lib().fbfc_recurrence_checkpoint_bytes(desc), x.device)
-        ws = self._workspace.take(lib().fbfc_recurrence_workspace_bytes(desc), x.device)
+        call = self._call(input, 3)
+        first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
+        self.output = _like(self.output, call)
+        self.state = self._state_like(self.state, call)
+        kept = self._checkpoints.take(call.checkpointBytes, call.device) if self.train else None
+        call.steps[2].data = self.output.data_ptr()
         self._forward = None
-        check(lib().fbfc_recurrence_forward(desc, _steps(x), _steps(gate), _ptr(self.bias), _ptr(state), _ptr(lengths),
-                                            _steps(self.output), _ptr(self.state), _ptr(kept), _ptr(ws), _stream()))
+        check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), first, sizes, call.refs[2],
+                                            self.state.data_ptr(), kept.data_ptr() if self.train else None,
+                                            self._workspace.take(call.workspaceBytes, call.device).data_ptr(), _stream()))
         if self.train:
-            self._forward = (x.shape, x.dtype, lengths, kept)
+            self._forward = (call.shape, call.dtype, lengths, kept)
         return self.output
 
     forward = updateOutput
 
     def step(self, input, state):
         """One token of each sequence: [x, gate] of (batch, nChannels); advances `state` in place and gives the output."""
-        if len(input) != 2:
-            raise ValueError("the input is [x, gate]")
-        x, gate = input
-        _check_activation(x, "x")
-        _check_activation(gate, "gate", x)
-        if x.dim() != 2 or x.size(1) != self.nChannels:
-            raise ValueError("x must be (batch, %d)" % self.nChannels)
+        call = self._call(input, 2)
         if state is None:
             raise TypeError("step needs the state that it advances")
-        self._check_state(state, "state", x.size(0))
-        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        tensors = [ctypes.byref(Steps(t.data_ptr(), t.stride(0), 0, t.stride(1))) for t in (x, gate, out)]
-        desc = RecurrenceDesc(x.size(0), self.nChannels, 1, TYPES[x.dtype])
-        check(lib().fbfc_recurrence_forward(ctypes.byref(desc), tensors[0], tensors[1], _ptr(self.bias), _ptr(state), None,
-                                            tensors[2], _ptr(state), None, None, _stream()))
-        return out
+        at = self._check_state(state, "state", call)
+        self.output = _like(self.output, call)
+        call.steps[2].data = self.output.data_ptr()
+        check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), at, None, call.refs[2], at, None,
+                                            None, _stream()))
+        return self.output
 
     def _backward(self, input, gradOutput, gradState, inputs, weights, scale):
-        x, gate, desc = self._inputs(input)
-        if self._forward is None or self._forward[:2] != (x.shape, x.dtype):
+        call = self._call(input, 3)
+        shape, dtype, lengths, kept = self._forward or (None, None, None, None)
+        if shape != call.shape or dtype != call.dtype or kept.device != call.device:
             raise ValueError("backward follows an updateOutput of the same inputs, not after evaluate()")
-        _check_activation(gradOutput, "gradOutput", x)
-        self._check_state(gradState, "gradState", x.size(0))
-        grads, first = [None, None], None
+        _check_activation(gradOutput, "gradOutput", call)
+        last = self._check_state(gradState, "gradState", call)
+        of = call.steps[5]
+        of.data = gradOutput.data_ptr()
+        of.stride_batch, of.stride_step, of.stride_channel = gradOutput.stride()
+        grads, first = (None, None), None
         if inputs:
-            old = self.gradInput or [None, None]
-            self.gradInput = [_like(old[0], x), _like(old[1], x)]
-            grads = [_steps(t) for t in self.gradInput]
-            if self.gradState is None or self.gradState.size(0) != x.size(0) or self.gradState.device != x.device:
-                self.gradState = torch.empty(x.size(0), self.nChannels, device=x.device)
-            first = self.gradState
-        ws = self._workspace.take(lib().fbfc_recurrence_workspace_bytes(desc), x.device)
-        check(lib().fbfc_recurrence_backward(desc, _steps(x), _steps(gate), _ptr(self.bias), _ptr(self._forward[2]),
-                                             _ptr(self._forward[3]), _steps(gradOutput), _ptr(gradState), *grads,
-                                             _ptr(self.gradBias if weights else None), scale, _ptr(first), _ptr(ws), _stream()))
+            old = self.gradInput or (None, None)
+            self.gradInput = [_like(old[0], call), _like(old[1], call)]
+            call.steps[3].data, call.steps[4].data = (t.data_ptr() for t in self.gradInput)
+            grads = call.refs[3:5]
+            self.gradState = self._state_like(self.gradState, call)
+            first = self.gradState.data_ptr()
+        check(lib().fbfc_recurrence_backward(call.desc, *call.refs[:2], self.bias.data_ptr(), _ptr(lengths), kept.data_ptr(),
+                                             call.refs[5], last, *grads,
+                                             self.gradBias.data_ptr() if weights else None, scale, first,
+                                             self._workspace.take(call.workspaceBytes, call.device).data_ptr(), _stream()))
 
     def updateGradInput(self, input, gradOutput, gradState=None):
         """[gradient of x, gradient of gate]; self.gradState is the gradient of the state before the first step.  `gradState`:
@@ -173,6 +195,34 @@ class GatedLinearRecurrence:
         """updateGradInput and accGradParameters in one pass over the inputs."""
         self._backward(input, gradOutput, gradState, True, True, scale)
         return self.gradInput
+
+
+class _NormCall:
+    """What calls of the norms on inputs of one signature share: checked sizes and descriptors."""
+
+    def __init__(self, net, input):
+        residual = input[0]
+        _check_activation(residual, "residual")
+        if residual.dim() < 1 or residual.size(-1) != net.nChannels:
+            raise ValueError("residual must have %d channels last" % net.nChannels)
+        for t, name in zip(input[1:], net._names[1:]):
+            _check_activation(t, name, residual)
+        self.shape, self.dtype, self.device, self.index = residual.shape, residual.dtype, residual.device, residual.device.index
+        self.desc = ctypes.byref(ResidualNormDesc(residual.numel() // net.nChannels, net.nChannels, TYPES[residual.dtype], net.eps))
+        self.workspaceBytes = lib().fbfc_residual_norm_workspace_bytes(self.desc)
+        # residual, branch, gate; output, normed; their gradients; the inputs' gradients
+        self.rows = [Rows(0, net.nChannels) for _ in range(10)]
+        self.refs = [ctypes.byref(r) for r in self.rows]
+        for rows, t, name in zip(self.rows, input, net._names):
+            rows.stride = net._row_stride(t, name)
+        self.inputs = self.refs[:len(input)] + [None] * (3 - len(input))
+
+    def at(self, i, t):
+        """Descriptor i, now of tensor t; None for an absent one."""
+        if t is None:
+            return None
+        self.rows[i].data = t.data_ptr()
+        return self.refs[i]
 
 
 class GatedResidualNorm:
@@ -201,6 +251,8 @@ class GatedResidualNorm:
         self.gradPostWeight, self.gradScale, self.gradPreWeight = zero(branch), zero(branch), zero(norm)
         self.output, self.gradInput = None, None
         self._workspace = Workspace()
+        self._names = ("residual", "branch", "gate")[:1 + self.hasBranch + self.hasGate]
+        self._signature = self._last = None   # of the last inputs, and what their calls share
 
     def parameters(self):
         pairs = [(self.postWeight, self.gradPostWeight), (self.scale, self.gradScale), (self.preWeight, self.gradPreWeight)]
@@ -210,69 +262,70 @@ class GatedResidualNorm:
         for g in self.parameters()[1]:
             g.zero_()
 
-    # rows of a tensor for the C ABI; None is an absent one
-    def _rows(self, t, name):
-        if t is None:
-            return None
+    # the stride between the rows of a tensor
+    def _row_stride(self, t, name):
+        if t.is_contiguous():
+            return self.nChannels
         try:
             t = t.view(-1, self.nChannels)
         except RuntimeError:
             raise ValueError("%s must be rows of channels, one stride apart" % name) from None
         if self.nChannels > 1 and t.stride(1) != 1:
             raise ValueError("the channels of %s must lie side by side" % name)
-        return ctypes.byref(Rows(t.data_ptr(), t.stride(0)))
+        return t.stride(0)
 
-    def _inputs(self, input):
-        names = ("residual", "branch", "gate")[:1 + self.hasBranch + self.hasGate]
+    def _call(self, input):
         if isinstance(input, torch.Tensor):
             input = [input]
-        if len(input) != len(names):
-            raise ValueError("the input is [%s]" % ", ".join(names))
-        residual = input[0]
-        _check_activation(residual, "residual")
-        if residual.dim() < 1 or residual.size(-1) != self.nChannels:
-            raise ValueError("residual must have %d channels last" % self.nChannels)
-        for t, name in zip(input[1:], names[1:]):
-            _check_activation(t, name, residual)
-        desc = ResidualNormDesc(residual.numel() // self.nChannels, self.nChannels, TYPES[residual.dtype], self.eps)
-        return ctypes.byref(desc), residual, [self._rows(t, n) for t, n in zip(input, names)] + [None] * (3 - len(names))
+        if len(input) != len(self._names):
+            raise ValueError("the input is [%s]" % ", ".join(self._names))
+        of = signature(*input)
+        if of != self._signature:
+            self._last, self._signature = _NormCall(self, input), of
+        call = self._last
+        check_current(call.index)
+        for rows, t in zip(call.rows, input):
+            rows.data = t.data_ptr()
+        return call, input
 
     def updateOutput(self, input):
-        desc, residual, rows = self._inputs(input)
-        old = self.output or [None, None]
+        call, input = self._call(input)
+        old = self.output or (None, None)
         # without a branch the first output is the caller's tensor, never one to write into
-        output = _like(old[0], residual) if self.hasBranch else None
-        normed = _like(old[1], residual) if self.hasNorm else None
-        check(lib().fbfc_residual_norm_forward(desc, *rows, _ptr(self.postWeight), _ptr(self.scale), _ptr(self.preWeight),
-                                               self._rows(output, "output"), self._rows(normed, "normed"), _stream()))
-        self.output = [output if self.hasBranch else residual, normed]
+        output = _like(old[0], call) if self.hasBranch else None
+        normed = _like(old[1], call) if self.hasNorm else None
+        check(lib().fbfc_residual_norm_forward(call.desc, *call.inputs, *self._weights(), call.at(3, output), call.at(4, normed),
+                                               _stream()))
+        self.output = [output if self.hasBranch else input[0], normed]
         return self.output
 
     forward = updateOutput
 
+    def _weights(self):
+        return [None if t is None else t.data_ptr() for t in (self.postWeight, self.scale, self.preWeight)]
+
     def _backward(self, input, gradOutput, inputs, weights, scale):
-        desc, residual, rows = self._inputs(input)
+        call, input = self._call(input)
         gr, gn = gradOutput
         if gr is None and gn is None:
             raise ValueError("gradOutput is [gradOutput, gradNormed], and one of them is needed")
         if gn is not None and not self.hasNorm:
             raise ValueError("there is no norm behind the block to have a gradient")
-        for t, name in ((gr, "gradOutput"), (gn, "gradNormed")):
+        for i, t, name in ((5, gr, "gradOutput"), (6, gn, "gradNormed")):
             if t is not None:
-                _check_activation(t, name, residual)
+                _check_activation(t, name, call)
+                call.rows[i].stride = self._row_stride(t, name)
         grads = [None] * 3
         if inputs:
             old = self.gradInput or [None] * 3
-            n = 1 + self.hasBranch + self.hasGate
-            self.gradInput = [_like(old[i], residual) for i in range(n)]
-            grads = [self._rows(t, "gradInput") for t in self.gradInput] + [None] * (3 - n)
+            self.gradInput = [_like(old[i], call) for i in range(len(input))]
+            grads[:len(input)] = [call.at(7 + i, t) for i, t in enumerate(self.gradInput)]
         ws, params = None, [None] * 3
         if weights:
-            ws = self._workspace.take(lib().fbfc_residual_norm_workspace_bytes(desc), residual.device)
-            params = [self.gradPostWeight, self.gradScale, self.gradPreWeight]
-        check(lib().fbfc_residual_norm_backward(desc, *rows, _ptr(self.postWeight), _ptr(self.scale), _ptr(self.preWeight),
-                                                self._rows(gr, "gradOutput"), self._rows(gn, "gradNormed"), *grads,
-                                                *map(_ptr, params), scale, _ptr(ws), _stream()))
+            ws = self._workspace.take(call.workspaceBytes, call.device).data_ptr()
+            params = [None if t is None else t.data_ptr() for t in (self.gradPostWeight, self.gradScale, self.gradPreWeight)]
+        check(lib().fbfc_residual_norm_backward(call.desc, *call.inputs, *self._weights(), call.at(5, gr), call.at(6, gn), *grads,
+                                                *params, scale, ws, _stream()))
 
     def updateGradInput(self, input, gradOutput):
         self._backward(input, gradOutput, True, False, 1.0)

@@ -13,7 +13,21 @@ def _ptr(t):
 
 
 def _stream():
-    return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    # the address alone: torch.cuda.current_stream() makes an object for it, which took 2.5 us of a call of 8.7 us
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+
+
+def signature(*tensors):
+    """What a call's argument checks and descriptors depend on: equal signatures need neither again."""
+    try:
+        return [(t.shape, t.stride(), t.dtype, t.device) for t in tensors]
+    except AttributeError:
+        raise TypeError("CUDA tensors are needed") from None
+
+
+def check_current(index):
+    if torch.cuda.current_device() != index:
+        raise ValueError("the tensors are not on the current device")
 
 
 def _check_tensor(t, name, ndim=None, strided=False):
