@@ -14,7 +14,7 @@
 //
 // Bound by memory: a forward pass reads three rows and writes two, a backward pass reads five and writes three.  A row
 // stays in registers from its first load to its last store, with all its loads issued before the first sum.  Rows of up
-// to 64 vectors of 16 bytes take 8 to 64 lanes, and longer ones a workgroup, whose wavefronts exchange their sums through
+// to 1024 channels take 8 to 64 lanes, and longer ones a workgroup, whose wavefronts exchange their sums through
 // the LDS with one barrier a sum.  The workgroups walk over the rows, so that the weights and the sums of the weights'
 // gradients stay in registers too; these are then added over the workgroups in a fixed order by a second kernel.
 #include <hip/hip_runtime.h>
@@ -372,8 +372,8 @@ __global__ __launch_bounds__(kSumThreads) void norm_weights_kernel(NormArgs a, i
     if (a.grad_pre != nullptr) a.grad_pre[at] = s * a.factor;
 }
 
-// How a row is laid over lanes: `lanes` 8 to 64 (several rows a workgroup of 256) or the whole workgroup (`wide`),
-// `values` of a row in each lane.
+// How a row is laid over lanes: 8 to 64 of them (several rows a workgroup of 256), or the whole workgroup (`wide`), each
+// with `vectors` of 16 bytes.
 struct RowShape {
     int lanes, vectors, threads;
     bool wide;
@@ -386,19 +386,24 @@ static RowShape row_shape(long rows, int channels, int type, bool backward)
     const int need = (channels + vec - 1) / vec;
     RowShape r;
     r.vectors = 1;
-    r.wide = need > 64;
+    // few rows: 16 bytes a lane, the shortest way through a row; many: up to 16 values a lane, and no barriers up to 1024 channels
+    const bool few = rows < 512;
+    r.wide = need > (few ? 64 : 1024 / vec);
     if (!r.wide) {
         r.lanes = need <= 8 ? 8 : need <= 16 ? 16 : need <= 32 ? 32 : 64;
+        r.vectors = need <= 64 ? 1 : 16 / vec;
         r.threads = 256;
     } else {
-        // many rows: 16 values a lane, fewer wavefronts to a barrier; few: 16 bytes a lane, the shortest way through a row
-        r.vectors = rows < 512 && need <= 1024 ? 1 : 16 / vec;
+        r.vectors = few && need <= 1024 ? 1 : 16 / vec;
         r.lanes = ((need + r.vectors - 1) / r.vectors + 63) / 64 * 64;
         r.threads = r.lanes;
     }
-    const long blocks = r.wide ? rows : (rows + 256 / r.lanes - 1) / (256 / r.lanes);
-    // what 256 CUs hold: forward 2048 threads each, backward, with twice the registers, half as many wavefronts
-    const long most = backward ? (r.threads > 512 ? 256 : 256L * (512 / r.threads)) : 256L * (2048 / r.threads);
+    const int side = r.wide ? 1 : 256 / r.lanes;
+    const long blocks = (rows + side - 1) / side;
+    // Workgroups: 1024 threads on each of 256 CUs, backward, with twice the registers, 512.  (3001 rows of 1000 channels
+    // in 32 bits, backward: 512 workgroups 30.7 us, as few as share the rows evenly, 376, 35.6 us, 751 37.7 us.)
+    const int held = (backward ? 512 : 1024) / r.threads;
+    const long most = 256L * (held > 0 ? held : 1);
     r.groups = blocks < most ? blocks : most;
     return r;
 }
@@ -422,7 +427,8 @@ static hipError_t forward_typed(const NormArgs &a, const RowShape &r, hipStream_
     } else if (r.lanes == 8) FBFC_LAUNCH((norm_forward_kernel<T, 8, 1>), grid, block, 0, s, a);
     else if (r.lanes == 16) FBFC_LAUNCH((norm_forward_kernel<T, 16, 1>), grid, block, 0, s, a);
     else if (r.lanes == 32) FBFC_LAUNCH((norm_forward_kernel<T, 32, 1>), grid, block, 0, s, a);
-    else FBFC_LAUNCH((norm_forward_kernel<T, 64, 1>), grid, block, 0, s, a);
+    else if (r.vectors == 1) FBFC_LAUNCH((norm_forward_kernel<T, 64, 1>), grid, block, 0, s, a);
+    else FBFC_LAUNCH((norm_forward_kernel<T, 64, 16 / V>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
@@ -439,7 +445,8 @@ static hipError_t backward_typed(const NormArgs &a, const RowShape &r, hipStream
     } else if (r.lanes == 8) FBFC_LAUNCH((norm_backward_kernel<T, 8, 1>), grid, block, 0, s, a);
     else if (r.lanes == 16) FBFC_LAUNCH((norm_backward_kernel<T, 16, 1>), grid, block, 0, s, a);
     else if (r.lanes == 32) FBFC_LAUNCH((norm_backward_kernel<T, 32, 1>), grid, block, 0, s, a);
-    else FBFC_LAUNCH((norm_backward_kernel<T, 64, 1>), grid, block, 0, s, a);
+    else if (r.vectors == 1) FBFC_LAUNCH((norm_backward_kernel<T, 64, 1>), grid, block, 0, s, a);
+    else FBFC_LAUNCH((norm_backward_kernel<T, 64, 16 / V>), grid, block, 0, s, a);
     return hipGetLastError();
 }
 
