@@ -65,7 +65,7 @@ __host__ __device__ __forceinline__ Shape shape_of(int batch, int channels, long
     s.waves = runs < kWaves ? (int)runs : kWaves;
     if (s.waves < 1) s.waves = 1;
     s.blocks = (channels + kLanes * v - 1) / (kLanes * v);
-    s.tiles = (int)((runs + s.waves - 1) / s.waves);  // recurrence_fits(): tiles * cols is below 2^31
+    s.tiles = (int)((runs + s.waves - 1) / s.waves);  // recurrence_fits()
     s.cols = batch * s.blocks;
     s.chain = s.tiles > 1 && s.cols < kGroups;
     return s;
@@ -326,8 +326,8 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
     const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    unsigned ticket = blockIdx.x;
-    const unsigned all = (unsigned)s.tiles * s.cols;
+    unsigned long ticket = blockIdx.x;
+    const unsigned long all = (unsigned long)s.tiles * s.cols;
     if (s.chain) {
         if (threadIdx.x == 0) given = draw(ch);
         __syncthreads();
@@ -337,7 +337,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
     fill_runs<V>(sS, s.waves, 0.0f);
     float carry[V];  // in the first wavefront: the state before the tile
     for (int turn = 0; ticket < all; turn ^= 1, ticket = s.chain ? all : ticket + s.cols) {
-        const int order = ticket / (unsigned)s.cols, col = ticket % (unsigned)s.cols, tile = order;
+        const int order = (int)(ticket / (unsigned)s.cols), col = (int)(ticket % (unsigned)s.cols), tile = order;
         const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
         const long len = length_of(a.lengths, b, steps);
         const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
@@ -447,8 +447,8 @@ __global__ __launch_bounds__(kLanes *kWaves, 2) void recurrence_backward_kernel(
     const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    unsigned ticket = blockIdx.x;
-    const unsigned all = (unsigned)s.tiles * s.cols;
+    unsigned long ticket = blockIdx.x;
+    const unsigned long all = (unsigned long)s.tiles * s.cols;
     if (s.chain) {
         if (threadIdx.x == 0) given = draw(ch);
         __syncthreads();
@@ -459,7 +459,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 2) void recurrence_backward_kernel(
     fill_runs<V>(sR, s.waves, 0.0f);
     float carry[V];  // in the first wavefront: a_{t+1} u_{t+1} behind the tile
     for (int turn = 0; ticket < all; turn ^= 1, ticket = s.chain ? all : ticket + s.cols) {
-        const int order = ticket / (unsigned)s.cols, col = ticket % (unsigned)s.cols, tile = s.tiles - 1 - order;
+        const int order = (int)(ticket / (unsigned)s.cols), col = (int)(ticket % (unsigned)s.cols), tile = s.tiles - 1 - order;
         const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
         const long len = length_of(a.lengths, b, steps);
         const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
@@ -708,10 +708,13 @@ size_t recurrence_workspace_bytes(int batch, int channels, long steps)
     return most + recurrence_checkpoint_bytes(batch, channels, steps);  // the sums of the gate's gradients of each tile
 }
 
+// One launch has fewer than 2^32 threads, of up to 512 in a workgroup; the kernel that adds up the bias's gradient has 64 for
+// each channel.
 bool recurrence_fits(int batch, int channels, long steps)
 {
     const long tiles = (steps + kRun * kWaves - 1) / (kRun * kWaves) + 1, cols = (channels + kLanes - 1L) / kLanes * batch;
-    return cols < 1L << 31 && tiles < (1L << 31) / (cols < 1 ? 1 : cols);
+    return channels <= 1 << 25 && (long)batch * channels < 1L << 31 && cols < 1L << 23 &&
+           (cols >= kGroups ? tiles < 1L << 31 : tiles < (1L << 23) / (cols < 1 ? 1 : cols));
 }
 
 static hipError_t clear_chain(const RecArgs &a, const Shape &s, int v, hipStream_t stream)

@@ -24,6 +24,13 @@ bool type_ok(int t) { return t == FBFC_F32 || t == FBFC_BF16 || t == FBFC_F16; }
 size_t type_bytes(int t) { return t == FBFC_F32 ? 4 : 2; }
 bool aligned(const void *p, size_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
+// Whether every pointer of 32-bit values is aligned to them (a null one is).
+template <typename... P>
+bool aligned32(const P *...p)
+{
+    return (aligned(p, 4) && ...);
+}
+
 // A stretch of memory that a call reads or writes.
 struct Range {
     uintptr_t begin, end;
@@ -276,6 +283,8 @@ static int norm_check_weights(const fbfc::NormArgs &a, bool normed)
     if (a.branch.data != nullptr && (a.post == nullptr || a.scale == nullptr))
         return fail(FBFC_ERR_INVALID_ARGUMENT, "a branch needs its norm's weight and its scale");
     if (normed && a.pre == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "the norm behind the block needs its weight");
+    if (!aligned32(a.post, a.scale, a.pre, a.grad_post, a.grad_scale, a.grad_pre))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "weights must be aligned to 4 bytes");
     return FBFC_OK;
 }
 
@@ -362,7 +371,7 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *d, const fbfc_row
             if ((rc = norm_check_rows(d, *r, false)) != FBFC_OK) return rc;
         for (const fbfc::Rows *r : {&a.grad_residual, &a.grad_branch, &a.grad_gate})
             if ((rc = norm_check_rows(d, *r, true)) != FBFC_OK) return rc;
-        if (weights && workspace == nullptr)
+        if (weights && (workspace == nullptr || !aligned(workspace, 4)))
             return fail(FBFC_ERR_INVALID_ARGUMENT, "the gradients of the weights need the workspace");
     } else if ((grad_post_weight != nullptr && scale == nullptr) || (grad_scale != nullptr && post_weight == nullptr)) {
         return fail(FBFC_ERR_INVALID_ARGUMENT, "a branch needs its norm's weight and its scale");
@@ -443,6 +452,8 @@ int fbfc_recurrence_forward(const fbfc_recurrence_desc *d, const fbfc_steps *inp
     a.checkpoints = checkpoints;
     a.workspace = static_cast<unsigned char *>(workspace);
     if (d->batch == 0) return FBFC_OK;
+    if (!aligned32(gate_bias, state_in, lengths, state_out, checkpoints))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "states, lengths and the bias must be aligned to 4 bytes");
     if (d->steps > 0) {
         if (a.x.data == nullptr || a.gate.data == nullptr || a.y.data == nullptr)
             return fail(FBFC_ERR_INVALID_ARGUMENT, "input, gate and output are needed");
@@ -481,6 +492,8 @@ int fbfc_recurrence_backward(const fbfc_recurrence_desc *d, const fbfc_steps *in
     a.grad_bias = grad_gate_bias;
     a.factor = factor;
     a.workspace = static_cast<unsigned char *>(workspace);
+    if (!aligned32(gate_bias, lengths, checkpoints, grad_state_out, grad_gate_bias, grad_state_in))
+        return fail(FBFC_ERR_INVALID_ARGUMENT, "states, lengths and the bias must be aligned to 4 bytes");
     if (d->batch > 0 && d->steps > 0) {
         if (a.x.data == nullptr || a.gate.data == nullptr || a.y.data == nullptr || checkpoints == nullptr)
             return fail(FBFC_ERR_INVALID_ARGUMENT, "input, gate, the output's gradient and the checkpoints are needed");

@@ -133,7 +133,8 @@ class GatedLinearRecurrence:
     def updateOutput(self, input, state=None, lengths=None):
         call = self._call(input, 3)
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
-        self.output = _like(self.output, call)
+        # an input that is this module's last output keeps its values, which backward reads
+        self.output = _like(None if input[0] is self.output or input[1] is self.output else self.output, call)
         self.state = self._state_like(self.state, call)
         kept = self._checkpoints.take(call.checkpointBytes, call.device) if self.train else None
         call.steps[2].data = self.output.data_ptr()
@@ -208,7 +209,8 @@ class _NormCall:
         for t, name in zip(input[1:], net._names[1:]):
             _check_activation(t, name, residual)
         self.shape, self.dtype, self.device, self.index = residual.shape, residual.dtype, residual.device, residual.device.index
-        self.desc = ctypes.byref(ResidualNormDesc(residual.numel() // net.nChannels, net.nChannels, TYPES[residual.dtype], net.eps))
+        self.sizes = ResidualNormDesc(residual.numel() // net.nChannels, net.nChannels, TYPES[residual.dtype], net.eps)
+        self.desc = ctypes.byref(self.sizes)
         self.workspaceBytes = lib().fbfc_residual_norm_workspace_bytes(self.desc)
         # residual, branch, gate; output, normed; their gradients; the inputs' gradients
         self.rows = [Rows(0, net.nChannels) for _ in range(10)]
@@ -284,14 +286,16 @@ class GatedResidualNorm:
             self._last, self._signature = _NormCall(self, input), of
         call = self._last
         check_current(call.index)
+        call.sizes.eps = self.eps
         for rows, t in zip(call.rows, input):
             rows.data = t.data_ptr()
         return call, input
 
     def updateOutput(self, input):
         call, input = self._call(input)
-        old = self.output or (None, None)
-        # without a branch the first output is the caller's tensor, never one to write into
+        # an input that is one of this module's last outputs keeps its values, which backward reads; without a branch the
+        # first output is the caller's tensor, never one to write into
+        old = [None if any(t is x for x in input) else t for t in self.output or (None, None)]
         output = _like(old[0], call) if self.hasBranch else None
         normed = _like(old[1], call) if self.hasNorm else None
         check(lib().fbfc_residual_norm_forward(call.desc, *call.inputs, *self._weights(), call.at(3, output), call.at(4, normed),

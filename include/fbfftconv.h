@@ -342,7 +342,8 @@ int fbfc_acc_grad_parameters_bias_noalloc(const float *grad_output, float *grad_
 /* Training and serving operators ---------------------------------------------------
  * What a network around the convolution layers needs besides them.  None has a counterpart in the
  * reference.  Activations may have 32 or 16 bits; parameters of the layers, their gradients and every
- * sum have 32. */
+ * sum have 32.  Every call works on the current device, with memory and a stream of that device, allocates
+ * nothing but where it says so, and may be captured into a graph. */
 enum { FBFC_F32 = 0, FBFC_BF16 = 1, FBFC_F16 = 2 };
 
 /* One AdamW step over all the parameters of a network, in one launch:
@@ -364,7 +365,8 @@ enum { FBFC_F32 = 0, FBFC_BF16 = 1, FBFC_F16 = 2 };
  * Tensors may begin anywhere (aligned to their type) and be empty; a parameter or a state that shares memory with
  * another tensor is refused.  One step at a time; the step counts itself, so that a step captured into a graph is a
  * new step at each replay (with the captured lr, weight_decay and grad_scale).  An optimizer works on the device
- * that was current when it was made. */
+ * that was current when it was made; create allocates a table there, destroy frees it (no step may then be running or waiting in
+ * a graph). */
 typedef struct {
     int param_type, grad_type;   /* FBFC_F32, FBFC_BF16 or FBFC_F16 */
     int state_bits;              /* 32 or 8 */
@@ -434,7 +436,7 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_
  * `lengths` (null: all of full length) holds the number of steps of each sequence, on the device, taken as between 0
  * and `steps`: what lies behind them is not read, and the output and the gradients there are zero; state_out is the
  * state behind the last of them.  No steps or no sequences is no error: the state passes through.  One step is the form
- * for serving: one launch, and no workspace.
+ * for serving: one launch, and no workspace.  Up to 2^25 channels and 2^31 channels of all sequences.
  *
  * `checkpoints` (fbfc_recurrence_checkpoint_bytes bytes, null where no gradient follows) keeps the state before each
  * 128 steps for backward, which takes the same descriptor, inputs and lengths.  backward assigns each gradient that is

@@ -83,6 +83,67 @@ int fbfc_acc_grad_parameters_bias_strided(const float *grad_output, float *grad_
 int fbfc_acc_grad_parameters_bias_noalloc(const float *grad_output, float *grad_bias, float scale,
                                           int batch, int planes, int h, int w, void *stream);
 
+/* training and serving operators */
+enum { FBFC_F32 = 0, FBFC_BF16 = 1, FBFC_F16 = 2 };
+typedef struct {
+    int param_type, grad_type;
+    int state_bits;
+    unsigned seed;
+    double beta1, beta2, eps;
+} fbfc_adamw_config;
+typedef struct {
+    void *param;
+    const void *grad;
+    long n;
+} fbfc_adamw_tensor;
+typedef struct fbfc_adamw fbfc_adamw;
+long fbfc_adamw_state_elements(const fbfc_adamw_tensor *tensors, int count);
+int fbfc_adamw_create(const fbfc_adamw_config *config, const fbfc_adamw_tensor *tensors, int count, void *m, void *v,
+                      float *m_scale, float *v_scale, fbfc_adamw **opt);
+int fbfc_adamw_destroy(fbfc_adamw *opt);
+int fbfc_adamw_step(fbfc_adamw *opt, double lr, double weight_decay, float grad_scale, void *stream);
+int fbfc_adamw_set_step(fbfc_adamw *opt, long steps, void *stream);
+int fbfc_adamw_get_step(fbfc_adamw *opt, long *steps, void *stream);
+typedef struct {
+    long rows;
+    int channels;
+    int type;
+    float eps;
+} fbfc_residual_norm_desc;
+typedef struct {
+    void *data;
+    long stride;
+} fbfc_rows;
+int fbfc_residual_norm_forward(const fbfc_residual_norm_desc *desc, const fbfc_rows *residual, const fbfc_rows *branch,
+                               const fbfc_rows *gate, const float *post_weight, const float *scale,
+                               const float *pre_weight, const fbfc_rows *output, const fbfc_rows *normed, void *stream);
+size_t fbfc_residual_norm_workspace_bytes(const fbfc_residual_norm_desc *desc);
+int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_rows *residual, const fbfc_rows *branch,
+                                const fbfc_rows *gate, const float *post_weight, const float *scale,
+                                const float *pre_weight, const fbfc_rows *grad_output, const fbfc_rows *grad_normed,
+                                const fbfc_rows *grad_residual, const fbfc_rows *grad_branch, const fbfc_rows *grad_gate,
+                                float *grad_post_weight, float *grad_scale, float *grad_pre_weight, float factor,
+                                void *workspace, void *stream);
+typedef struct {
+    int batch, channels;
+    long steps;
+    int type;
+} fbfc_recurrence_desc;
+typedef struct {
+    void *data;
+    long stride_batch, stride_step, stride_channel;
+} fbfc_steps;
+size_t fbfc_recurrence_checkpoint_bytes(const fbfc_recurrence_desc *desc);
+size_t fbfc_recurrence_workspace_bytes(const fbfc_recurrence_desc *desc);
+int fbfc_recurrence_forward(const fbfc_recurrence_desc *desc, const fbfc_steps *input, const fbfc_steps *gate,
+                            const float *gate_bias, const float *state_in, const int *lengths, const fbfc_steps *output,
+                            float *state_out, float *checkpoints, void *workspace, void *stream);
+int fbfc_recurrence_backward(const fbfc_recurrence_desc *desc, const fbfc_steps *input, const fbfc_steps *gate,
+                             const float *gate_bias, const int *lengths, const float *checkpoints,
+                             const fbfc_steps *grad_output, const float *grad_state_out, const fbfc_steps *grad_input,
+                             const fbfc_steps *grad_gate, float *grad_gate_bias, float factor, float *grad_state_in,
+                             void *workspace, void *stream);
+
 /* from the HIP build of cutorch (libTHC): the stream the current Torch state launches on */
 typedef struct THCState THCState;
 void *THCState_getCurrentStream(THCState *state);

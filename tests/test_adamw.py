@@ -351,3 +351,25 @@ def test_module_refusals_and_modules():
     net.updateOutput(x)
     net.accGradParameters(x, torch.randn(2, 5, 13, 13, device="cuda"))
     Plain(opt).step(opt.step)
+
+
+@pytest.mark.gpu
+def test_more_than_32_bits_of_parameters():
+    """2.2 thousand million parameters in one tensor: its end steps as a tensor of its own does, in both forms of states."""
+    from fbcunn_amd import optim
+    n, cut = (1 << 31) + (1 << 27) + 77, (1 << 31) + (1 << 27) - 2048     # the cut is a whole block
+    gen = torch.Generator("cuda").manual_seed(1)
+    p, g = (torch.empty(n, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    q, h = p[cut:].clone(), g[cut:].clone()
+    opt, part = optim.AdamW([p], [g], **HYPER), optim.AdamW([q], [h], **HYPER)
+    opt.step(), part.step()
+    assert torch.equal(p[cut:], q) and torch.equal(opt.v[cut:], part.v)
+    del opt, part
+    opt = optim.AdamW([p], [g], stateBits=8, **HYPER)
+    before = p[cut:].float()
+    opt.step()
+    value = opt.m[cut:].float().view(-1, 256) * opt.mScale[cut // 256:, None]
+    want = torch.nn.functional.pad(h.float() * (1 - 0.9), (0, -h.numel() % 256)).view(-1, 256)
+    assert bool(((value - want).abs() <= 2.0 ** -3 * want.abs() + opt.mScale[cut // 256:, None] * 2.0 ** -9).all())   # one spacing
+    assert not torch.equal(p[cut:].float(), before)
+    assert len(opt.m[cut:].view(torch.uint8).unique()) > 100

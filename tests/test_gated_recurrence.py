@@ -439,3 +439,30 @@ def test_module_refusals():
     net.updateOutput([x, x])
     with pytest.raises(ValueError):
         net.backward([x, x], x)
+
+
+def test_misaligned_states_and_oversized_shapes_are_refused():
+    for kw in (dict(bias=0x1002), dict(state_in=0x1001), dict(lengths=0x1002), dict(state_out=0x1002), dict(checkpoints=0x1003)):
+        rc, message = _forward(**kw)
+        assert rc == _lib.ERR_INVALID_ARGUMENT and "4 bytes" in message
+    for kw in (dict(bias=0x1002), dict(lengths=0x1001), dict(checkpoints=0x1002), dict(gstate=0x1002), dict(gb=0x1002), dict(gstate_in=0x1001)):
+        rc, message = _backward(**kw)
+        assert rc == _lib.ERR_INVALID_ARGUMENT and "4 bytes" in message
+    # one launch has fewer than 2^32 threads
+    for kw in (dict(channels=(1 << 25) + 1), dict(batch=1 << 16, channels=1 << 15), dict(batch=1 << 23, channels=1),
+               dict(batch=1, channels=64, steps=1 << 31)):
+        assert _forward(**kw)[0] == _lib.ERR_UNSUPPORTED_SIZE, kw
+
+
+@pytest.mark.gpu
+def test_own_output_as_input_keeps_its_values():
+    """A module whose last output is its next input: the output goes elsewhere, and backward sees the input."""
+    net, x, gate, gy, _, _ = _data(2, 200, 12, torch.float32, 17)
+    y = net.updateOutput([x, gate])
+    kept = y.clone()
+    z = net.updateOutput([y, gate])
+    assert z is not y and torch.equal(y, kept)
+    net.backward([y, gate], gy)
+    want = _plain(kept, gate, net.bias, None, None, gy, None)
+    _check(z, want["output"], "output")
+    _check(net.gradInput[1], want["gradGate"], "gradGate")

@@ -382,3 +382,43 @@ def test_module_refusals_and_shapes():
         _net(16, "last", 1).backward([x, x, x], [x, x])
     with pytest.raises(_lib.FbfcError):
         _net(16385, "first", 1).updateOutput([torch.zeros(2, 16385, device="cuda")])
+
+
+def test_misaligned_weights_are_refused():
+    for kw in (dict(post=0x1002), dict(scale=0x1001), dict(pre=0x1002)):
+        for call in (_forward, _backward):
+            rc, message = call(**kw)
+            assert rc == _lib.ERR_INVALID_ARGUMENT and "4 bytes" in message
+    for kw in (dict(dpost=0x1002), dict(dscale=0x1002), dict(dpre=0x1002)):
+        assert _backward(**kw)[0] == _lib.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.gpu
+def test_own_output_as_residual_and_a_changed_eps():
+    """The next block's residual is this module's output: it keeps its values.  eps is read at each call."""
+    net = _net(48, "full", 1)
+    inputs, grads = _inputs((6, 48), "full", torch.float32, 5)
+    first = net.updateOutput(inputs)
+    kept = [t.clone() for t in first]
+    again = net.updateOutput([first[0], inputs[1], inputs[2]])
+    assert again[0] is not first[0] and torch.equal(first[0], kept[0])
+    _check(again[1], _plain(net, [kept[0], inputs[1], inputs[2]])["normed"], "normed")
+    wide = net.updateOutput(inputs)[1].clone()
+    net.eps = 1.0
+    assert not torch.equal(net.updateOutput(inputs)[1], wide)
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits():
+    """2.3 thousand million elements: the last rows as a tensor of their own, forward and backward."""
+    rows, channels = 140000, 16384
+    net, part = _net(channels, "ungated", 1), _net(channels, "ungated", 1)
+    gen = torch.Generator("cuda").manual_seed(2)
+    x, y = (torch.empty(rows, channels, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
+    net.updateOutput([x, y])
+    tail = [x[-64:], y[-64:]]
+    for a, b in zip(net.output, part.updateOutput(tail)):
+        assert torch.equal(a[-64:], b)
+    net.updateGradInput([x, y], [x, y])
+    for a, b in zip(net.gradInput, part.updateGradInput(tail, tail)):
+        assert torch.equal(a[-64:], b)
