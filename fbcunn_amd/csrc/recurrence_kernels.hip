@@ -100,7 +100,10 @@ constexpr int kAsk = 4;
 template <int V>
 __device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, int at, int col, int dir, int lane, float (&h)[V])
 {
-    const long cell = (long)kLanes * V, place = (long)col * cell + lane * V, row = (long)s.cols * cell;
+    const long cell = (long)kLanes * V, row = (long)s.cols * cell;
+    const unsigned *states = ch.states + col * cell;
+    const word64 *runs = ch.runs + col * cell;
+    const unsigned own = lane * V;
     int j = at + dir;  // the nearest of the tiles that are asked
     while (true) {
         unsigned state[kAsk][V];
@@ -111,8 +114,8 @@ __device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, int a
             k = k < 0 ? 0 : k < s.tiles ? k : s.tiles - 1;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                state[q][i] = __hip_atomic_load(ch.states + k * row + place + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-                run[q][i] = __hip_atomic_load(ch.runs + k * row + place + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                state[q][i] = __hip_atomic_load(states + k * row + (own + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                run[q][i] = __hip_atomic_load(runs + k * row + (own + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             }
         }
         int hit = -1, known = 0;  // the tile whose state is announced; how many before it have announced their runs
@@ -147,7 +150,7 @@ __device__ __forceinline__ void look_back(const Chain &ch, const Shape &s, int a
     for (j -= dir; j != at; j -= dir) {
         word64 run[V];
 #pragma unroll
-        for (int i = 0; i < V; ++i) run[i] = __hip_atomic_load(ch.runs + j * row + place + i, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        for (int i = 0; i < V; ++i) run[i] = __hip_atomic_load(runs + j * row + (own + i), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         fold<V>(h, run);
     }
 }
@@ -173,12 +176,15 @@ __device__ __forceinline__ void announce_state(const Chain &ch, const Shape &s, 
 // or before a lane, its loads are moved back to end with the row, so that no load has a condition, and an odd last channel
 // is then moved to its place.  DENSE: channels side by side, with an offset that fits 32 bits, so that the row's
 // address stays in scalar registers.
+//
+// Forward, a lane has 4 bytes of each row, two channels in 16 bits.  Backward it has one: with two, a wavefront needs 178
+// registers instead of 111, and one workgroup fits a CU where two do (131072 steps of 2048 channels in bf16: 752 us with two
+// channels, 662 with one; forward 393 with two and 425 with one).
 template <typename T, bool DENSE>
-constexpr int kLaneChannels = DENSE && sizeof(T) == 2 ? 2 : 1;  // 4 bytes a lane
+constexpr int kLaneChannels = DENSE && sizeof(T) == 2 ? 2 : 1;
 
-template <typename T, bool DENSE>
+template <typename T, bool DENSE, int V>
 struct LaneRows {
-    static constexpr int V = kLaneChannels<T, DENSE>;
     typedef typename std::conditional<DENSE, unsigned, long>::type Offset;
     const char *base;
     long st;             // bytes from row to row
@@ -340,7 +346,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
         const int order = (int)(ticket / (unsigned)s.cols), col = (int)(ticket % (unsigned)s.cols), tile = order;
         const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
         const long len = length_of(a.lengths, b, steps);
-        const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
+        const LaneRows<T, DENSE, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
         const bool whole = __all(c + V <= a.channels);
         float bias2[V];
 #pragma unroll
@@ -438,9 +444,9 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
 }
 
 template <typename T, bool DENSE>
-__global__ __launch_bounds__(kLanes *kWaves, 2) void recurrence_backward_kernel(RecArgs a, float *partial)
+__global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(RecArgs a, float *partial)
 {
-    constexpr int V = kLaneChannels<T, DENSE>;
+    constexpr int V = 1;
     __shared__ float sA[2][kWaves][kLanes * V], sS[2][kWaves][kLanes * V], sR[2][kWaves][kLanes * V], carried[kLanes * V];
     __shared__ unsigned given;
     const long steps = a.steps;
@@ -462,7 +468,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 2) void recurrence_backward_kernel(
         const int order = (int)(ticket / (unsigned)s.cols), col = (int)(ticket % (unsigned)s.cols), tile = s.tiles - 1 - order;
         const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
         const long len = length_of(a.lengths, b, steps);
-        const LaneRows<T, DENSE> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
+        const LaneRows<T, DENSE, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
             gxr(a.grad_x, b, c, a.channels), ggr(a.grad_gate, b, c, a.channels);
         const bool whole = __all(c + V <= a.channels);
         float bias2[V];
@@ -756,14 +762,13 @@ template <typename T>
 static hipError_t backward_typed(int type, const RecArgs &a, hipStream_t stream)
 {
     const bool side = dense(type, a);
-    const int v = side ? kLaneChannels<T, true> : 1;
-    const Shape s = shape_of(a.batch, a.channels, a.steps, v);
+    const Shape s = shape_of(a.batch, a.channels, a.steps, 1);
     float *partial = nullptr;
     if (a.grad_bias != nullptr)
         partial = reinterpret_cast<float *>(a.workspace + recurrence_workspace_bytes(a.batch, a.channels, a.steps) -
                                             recurrence_checkpoint_bytes(a.batch, a.channels, a.steps));
     if (s.chain) {
-        const hipError_t e = clear_chain(a, s, v, stream);
+        const hipError_t e = clear_chain(a, s, 1, stream);
         if (e != hipSuccess) return e;
     }
     const dim3 grid(s.chain ? s.tiles * s.cols : s.cols), block(s.waves * kLanes);
