@@ -10,7 +10,7 @@
 // once.  A run of steps maps a state h to A h + S, and two runs after each other to (A2 A1, A2 S1 + S2), so the
 // steps can be worked on side by side: a wavefront holds 16 steps of 64 lanes' channels in registers, a workgroup
 // of up to 8 wavefronts a tile of 128 steps, whose runs it joins through the LDS.  Then either one workgroup walks over the
-// tiles of its channels (where there are enough channels to fill the GPU), or every tile is a workgroup of its own and
+// tiles of its channels (where there are enough channels to fill the GPU, or two tiles), or every tile is a workgroup of its own and
 // the state goes from tile to tile through memory: a tile announces its (A, S) as soon as it has them, looks back for
 // the nearest state announced by a tile before it, and applies the (A, S) of those in between, in their order, so that the
 // result does not depend on how far it had to look.  Tiles are given out by a counter in the order in which they
@@ -31,9 +31,13 @@ namespace fbfc {
 constexpr int kRun = 16;     // steps of a wavefront
 constexpr int kWaves = 8;     // wavefronts of a workgroup, at most
 constexpr int kLanes = 64;
-// Workgroups that the GPU holds, two on each CU: as many columns or more are walked over by one workgroup each, fewer by
-// several, which hand the state from tile to tile.
-constexpr int kGroups = 512;
+// Columns (a sequence's block of channels) from which on one workgroup walks over all tiles of its column: with one on
+// each CU, handing the state from tile to tile gains nothing (256 columns of 12 tiles in 32 bits: 60 us walked over, 64
+// handed on; 4 tiles 21 and 28).  Below, tiles are worked on side by side where there are enough to make up for clearing the
+// announcements: 3 or more (16 columns in 32 bits: 2 tiles 7.4 us walked over and 10.8 handed on, 4 tiles 11.8 and 10.3, 12
+// tiles 31 and 10), or, with half of the CUs at work anyway, 5 (128 columns in bf16: 3 tiles 14.9 and 17.5, 4 tiles
+// 20.3 and 19.8, 12 tiles 54 and 39).
+constexpr int kGroups = 256;
 constexpr int kHead = 256;    // bytes of the workspace before the announcements
 constexpr float kLog2e = 1.44269504088896340736f;
 
@@ -67,7 +71,7 @@ __host__ __device__ __forceinline__ Shape shape_of(int batch, int channels, long
     s.blocks = (channels + kLanes * v - 1) / (kLanes * v);
     s.tiles = (int)((runs + s.waves - 1) / s.waves);  // recurrence_fits()
     s.cols = batch * s.blocks;
-    s.chain = s.tiles > 1 && s.cols < kGroups;
+    s.chain = s.cols < kGroups && s.tiles > (s.cols < kGroups / 2 ? 2 : 4);
     return s;
 }
 

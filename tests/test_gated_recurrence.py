@@ -393,9 +393,9 @@ def test_two_streams_at_once():
 
 
 @pytest.mark.gpu
-def test_offsets_beyond_32_bits():
+@pytest.mark.parametrize("T,D", [(70016, 32768), (140032, 16384)])    # one workgroup a column; tiles handed on
+def test_offsets_beyond_32_bits(T, D):
     """2.3 thousand million elements: the last tiles from the checkpoint before them, as a sequence of their own."""
-    T, D = 70016, 32768
     from fbcunn_amd import nn
     gen = torch.Generator("cuda").manual_seed(1)
     x, gate = (torch.empty(1, T, D, dtype=torch.bfloat16, device="cuda").normal_(generator=gen) for _ in range(2))
