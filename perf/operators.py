@@ -150,6 +150,10 @@ def _run_recurrence(case, s):
         if way == "forward":
             return [y, net.state]
         net.backward([s["x"], s["gate"]], s["gy"], gradState=s["gh"])
+        if s["gy"].dtype == torch.float32 and s["lengths"] is None:
+            # the plain form adds the state's gradient to the last step of these very gradients in place: the next pass on
+            # this state has to find them alike
+            s["gy"][:, -1] += s["gh"]
         return [y, net.state, net.gradInput[0], net.gradInput[1], net.gradState, net.gradBias]
     dt = s["x"].dtype
     x, z = s["x"].float(), s["gate"].float() + s["bias"]
