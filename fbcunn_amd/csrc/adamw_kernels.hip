@@ -16,6 +16,12 @@
 // thousandth a step, and a rounding to the nearest of numbers an eighth apart would never let it move.  The random numbers
 // are a hash of (seed, step, place), so a step can be repeated.  A positive v is never rounded to zero, where the
 // step m / sqrt(v) would have no bound.
+//
+// Measured: 40 million parameters of 160 tensors in 32 bits 222 us (5.05 TB/s, what a large copy reaches); 250 million with 16-bit
+// gradients and 8-bit states 726 us (4.84 TB/s); 25 million in bf16 with 8-bit states, unaligned, 62 us (4.06 TB/s; here
+// the arithmetic of the rounding counts, with divisions and roots rounded to half a unit 69 us).  Non-temporal stores,
+// 1024 to 4096 workgroups and 8 or 16 parameters in flight a lane are all within 3 %; a workgroup for each piece is
+// slower with 8-bit states (783 us).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
