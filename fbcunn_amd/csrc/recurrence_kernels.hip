@@ -46,7 +46,7 @@ constexpr int kHead = 256;    // bytes of the workspace before the announcements
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Announcements.  A word is announced once it differs from what the workspace is filled with, all ones (a NaN that
-// announce() never writes), so value and flag arrive together and no fence is needed.
+// announced() never gives), so value and flag arrive together and no fence is needed.
 typedef unsigned long long word64;
 constexpr unsigned kUnset = 0xFFFFFFFFu;
 constexpr word64 kUnset2 = ~0ull;
@@ -651,9 +651,8 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
 template <typename T, int V>
 __global__ __launch_bounds__(256) void recurrence_step_kernel(RecArgs a)
 {
-    const int per = (a.channels + V - 1) / V;
-    const long i = blockIdx.x * 256L + threadIdx.x;
-    if (i >= (long)a.batch * per) return;
+    const unsigned per = (a.channels + V - 1) / V, i = blockIdx.x * 256u + threadIdx.x;  // recurrence_fits(): below 2^31
+    if (i >= a.batch * per) return;
     const int b = (int)(i / per), c = (int)(i % per) * V;
     const bool live = a.steps > 0 && (a.lengths == nullptr || a.lengths[b] > 0);
     const long left = a.channels - c, at = (long)b * a.channels + c;
@@ -729,9 +728,13 @@ size_t recurrence_workspace_bytes(int batch, int channels, long steps)
 // each channel.
 bool recurrence_fits(int batch, int channels, long steps)
 {
-    const long tiles = (steps + kRun * kWaves - 1) / (kRun * kWaves) + 1, cols = (channels + kLanes - 1L) / kLanes * batch;
-    return channels <= 1 << 25 && (long)batch * channels < 1L << 31 && cols < 1L << 23 &&
-           (cols >= kGroups ? tiles < 1L << 31 : tiles < (1L << 23) / (cols < 1 ? 1 : cols));
+    const long tiles = (steps + kRun * kWaves - 1) / (kRun * kWaves) + 1, most = 1L << 23;
+    if (channels > 1 << 25 || (long)batch * channels >= 1L << 31 || tiles >= 1L << 31) return false;
+    for (int v = 1; v <= 2; ++v) {
+        const long cols = (channels + kLanes * v - 1L) / (kLanes * v) * batch;
+        if (cols >= most || (cols > 0 && cols < kGroups && tiles >= most / cols)) return false;  // a workgroup a column, or a tile
+    }
+    return true;
 }
 
 static hipError_t clear_chain(const RecArgs &a, const Shape &s, int v, hipStream_t stream)

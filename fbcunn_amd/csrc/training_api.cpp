@@ -394,7 +394,7 @@ static int recurrence_check_desc(const fbfc_recurrence_desc *d)
     if (d == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
     if (!type_ok(d->type)) return fail(FBFC_ERR_INVALID_ARGUMENT, "unknown type");
     if (d->batch < 0 || d->steps < 0 || d->channels < 1) return fail(FBFC_ERR_INVALID_ARGUMENT, "sizes must be positive");
-    if (d->batch > 0 && (d->steps > (1L << 40) || !fbfc::recurrence_fits(d->batch, d->channels, d->steps)))
+    if (d->steps > (1L << 40) || !fbfc::recurrence_fits(d->batch, d->channels, d->steps))
         return fail(FBFC_ERR_UNSUPPORTED_SIZE, "more sequences, channels and steps than one launch can take");
     return FBFC_OK;
 }

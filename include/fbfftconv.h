@@ -392,7 +392,8 @@ int fbfc_adamw_get_step(fbfc_adamw *opt, long *steps, void *stream);
  * row of `channels` values, with branch the block's result and rms(x) = sqrt(mean x^2 + eps):
  *     output = residual + scale * sigmoid(gate) * post_weight * branch / rms(branch)
  *     normed = pre_weight * output / rms(output)                the next block's input
- * computed in 32 bits from the inputs and rounded once: normed is the norm of the output before its rounding.  Parts
+ * computed in 32 bits from the inputs and rounded once: normed is the norm of the output before its rounding; a row whose
+ * squares add up to more than 32 bits hold has an infinite rms, and so a norm of zeros.  Parts
  * that are absent (a null pointer, or data null) drop out: without a gate the factor is one; without `normed` there is
  * no norm behind the block (the last one of a network); without a branch, and so without an output, normed is that of
  * the residual (before the first block).
@@ -434,9 +435,11 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_
  * planes of a convolution, are supported.  gate_bias has `channels` values, the states (batch, channels); null stands
  * for zeros.  state_out may be null, or be state_in.  The output may be one of the inputs with the same strides.
  * `lengths` (null: all of full length) holds the number of steps of each sequence, on the device, taken as between 0
- * and `steps`: what lies behind them is not read, and the output and the gradients there are zero; state_out is the
- * state behind the last of them.  No steps or no sequences is no error: the state passes through.  One step is the form
- * for serving: one launch, and no workspace.  Up to 2^25 channels and 2^31 channels of all sequences.
+ * and `steps`: what lies behind them has no effect, and the output and the gradients there are zero; state_out is the
+ * state behind the last of them.  The state moves by (1 - a_t) (input_t - state), which keeps the precision of 1 - a_t; an
+ * input that is infinite or NaN makes the state NaN from the next step on.  No steps or no sequences is no error: the
+ * state passes through.  One step is the form for serving: one launch, and no workspace.  Up to 2^25 channels and 2^31
+ * channels of all sequences.
  *
  * `checkpoints` (fbfc_recurrence_checkpoint_bytes bytes, null where no gradient follows) keeps the state before each
  * 128 steps for backward, which takes the same descriptor, inputs and lengths.  backward assigns each gradient that is
