@@ -25,6 +25,11 @@ def _check_activation(t, name, like=None):
             raise ValueError("%s is on another device" % name)
 
 
+def _check_device(t, parameters):
+    if any(p.device != t.device for tensors in parameters for p in tensors):
+        raise ValueError("the inputs are on another device than the parameters")
+
+
 def _like(old, t):
     """`old` where it can take what has the shape and the type of t, else a new tensor."""
     if old is not None and old.shape == t.shape and old.dtype == t.dtype and old.device == t.device:
@@ -32,15 +37,30 @@ def _like(old, t):
     return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
+def _apart(old, inputs):
+    """`old`, or None where one of the inputs lies in it: an input that is a module's last output, or a view of it, keeps
+    its values, which backward reads."""
+    if old is None:
+        return None
+    at = old.data_ptr()
+    end = at + old.nbytes
+    for t in inputs:
+        if at <= t.data_ptr() < end:
+            return None
+    return old
+
+
 class _RecurrenceCall:
     """What calls of the recurrence on inputs of one signature share: checked sizes and descriptors."""
 
-    def __init__(self, x, gate, channels, dims):
+    def __init__(self, net, x, gate, dims):
+        channels = net.nChannels
         _check_activation(x, "x")
         _check_activation(gate, "gate", x)
         if x.dim() != dims or x.size(-1) != channels:
             raise ValueError("x must be (%s%d)" % ("batch, steps, " if dims == 3 else "batch, ", channels))
         self.shape, self.dtype, self.device, self.index = x.shape, x.dtype, x.device, x.device.index
+        _check_device(x, net.parameters())
         self.batch, steps = x.size(0), x.size(1) if dims == 3 else 1
         desc = RecurrenceDesc(self.batch, channels, steps, TYPES[x.dtype])
         self.desc = ctypes.byref(desc)
@@ -59,10 +79,11 @@ class GatedLinearRecurrence:
     updateOutput takes [x, gate], both (batch, steps, nChannels), float32, bfloat16 or float16, of any strides, and gives the
     output, of the same shape; self.state is then the state behind the last step (batch, nChannels) in float32.
     `state`: the state before the first step, zeros where it is None.  `lengths`: an int32 CUDA tensor with the steps of each
-    sequence; behind them nothing is read, and outputs and gradients are zero.  backward (and its halves updateGradInput
-    and accGradParameters) follows an updateOutput of the same inputs, from which the module keeps the state before every
-    128 steps; after evaluate() it keeps none and cannot go backward.  step advances sequences by one token.  As in the
-    other modules the outputs are the module's own tensors, which its next call on inputs of the same shape writes again."""
+    sequence; what lies behind them has no effect, and outputs and gradients there are zero.  backward (and its halves
+    updateGradInput and accGradParameters) follows an updateOutput of the same inputs, from which the module keeps the
+    state before every 128 steps; after evaluate() it keeps none and cannot go backward.  step advances sequences by one
+    token.  As in the other modules the outputs are the module's own tensors, which its next call on inputs of the same
+    shape writes again, unless they are its inputs."""
 
     def __init__(self, nChannels, device="cuda"):
         if not isinstance(nChannels, int) or nChannels < 1:
@@ -96,7 +117,7 @@ class GatedLinearRecurrence:
         of = signature(x, gate)
         last, call = self._calls[dims]
         if last != of:
-            call = _RecurrenceCall(x, gate, self.nChannels, dims)
+            call = _RecurrenceCall(self, x, gate, dims)
             self._calls[dims] = (of, call)
         check_current(call.index)
         call.steps[0].data, call.steps[1].data = x.data_ptr(), gate.data_ptr()
@@ -133,8 +154,7 @@ class GatedLinearRecurrence:
     def updateOutput(self, input, state=None, lengths=None):
         call = self._call(input, 3)
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
-        # an input that is this module's last output keeps its values, which backward reads
-        self.output = _like(None if input[0] is self.output or input[1] is self.output else self.output, call)
+        self.output = _like(_apart(self.output, input), call)
         self.state = self._state_like(self.state, call)
         kept = self._checkpoints.take(call.checkpointBytes, call.device) if self.train else None
         call.steps[2].data = self.output.data_ptr()
@@ -154,7 +174,7 @@ class GatedLinearRecurrence:
         if state is None:
             raise TypeError("step needs the state that it advances")
         at = self._check_state(state, "state", call)
-        self.output = _like(self.output, call)
+        self.output = _like(_apart(self.output, input), call)
         call.steps[2].data = self.output.data_ptr()
         check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), at, None, call.refs[2], at, None,
                                             None, _stream()))
@@ -208,6 +228,7 @@ class _NormCall:
             raise ValueError("residual must have %d channels last" % net.nChannels)
         for t, name in zip(input[1:], net._names[1:]):
             _check_activation(t, name, residual)
+        _check_device(residual, net.parameters())
         self.shape, self.dtype, self.device, self.index = residual.shape, residual.dtype, residual.device, residual.device.index
         self.sizes = ResidualNormDesc(residual.numel() // net.nChannels, net.nChannels, TYPES[residual.dtype], net.eps)
         self.desc = ctypes.byref(self.sizes)
@@ -293,9 +314,8 @@ class GatedResidualNorm:
 
     def updateOutput(self, input):
         call, input = self._call(input)
-        # an input that is one of this module's last outputs keeps its values, which backward reads; without a branch the
-        # first output is the caller's tensor, never one to write into
-        old = [None if any(t is x for x in input) else t for t in self.output or (None, None)]
+        # without a branch the first output is the caller's tensor, never one to write into
+        old = [_apart(t, input) for t in self.output or (None, None)]
         output = _like(old[0], call) if self.hasBranch else None
         normed = _like(old[1], call) if self.hasNorm else None
         check(lib().fbfc_residual_norm_forward(call.desc, *call.inputs, *self._weights(), call.at(3, output), call.at(4, normed),

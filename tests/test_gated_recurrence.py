@@ -466,3 +466,43 @@ def test_own_output_as_input_keeps_its_values():
     want = _plain(kept, gate, net.bias, None, None, gy, None)
     _check(z, want["output"], "output")
     _check(net.gradInput[1], want["gradGate"], "gradGate")
+
+
+def test_sizes_that_no_launch_takes_are_refused_with_no_sequences_too():
+    # the sum of the bias's gradient has 64 threads for each channel, whatever the batch
+    assert _backward(batch=0, channels=1 << 27, gb=P)[0] == _lib.ERR_UNSUPPORTED_SIZE
+    # 256 columns of one channel a lane, and 128 of two: there each tile is a workgroup
+    assert _forward(batch=1, channels=64 * 256, steps=1 << 31, type=_lib.BF16)[0] == _lib.ERR_UNSUPPORTED_SIZE
+
+
+@pytest.mark.gpu
+def test_parameters_on_another_device_are_refused():
+    from fbcunn_amd import nn
+    net = nn.GatedLinearRecurrence(8, device="cpu")
+    x = torch.randn(2, 5, 8, device="cuda")
+    with pytest.raises(ValueError, match="another device"):
+        net.updateOutput([x, x])
+    with pytest.raises(ValueError, match="another device"):
+        net.step([x[:, 0], x[:, 0]], torch.zeros(2, 8, device="cuda"))
+
+
+@pytest.mark.gpu
+def test_views_of_the_own_output_as_input_keep_their_values():
+    from fbcunn_amd import nn
+    net, x, gate, gy, _, _ = _data(6, 6, 12, torch.float32, 18)
+    y = net.updateOutput([x, gate])
+    turned, kept = y.transpose(0, 1), y.clone()      # the same shape, other strides
+    z = net.updateOutput([turned, gate])
+    assert z is not y and torch.equal(y, kept)
+    net.backward([turned, gate], gy)
+    want = _plain(kept.transpose(0, 1), gate, net.bias, None, None, gy, None)
+    _check(z, want["output"], "output")
+    _check(net.gradInput[1], want["gradGate"], "gradGate")
+    # a token of two sequences, swapped
+    net = nn.GatedLinearRecurrence(12)
+    a, state = net.step([x[:2, 0], gate[:2, 0]], torch.zeros(2, 12, device="cuda")), torch.zeros(2, 12, device="cuda")
+    kept = a.clone()
+    b = net.step([a[:, :], a], state)
+    want = _plain(kept[:, None], kept[:, None], net.bias, None, None, kept[:, None], None)
+    assert b is not a and torch.equal(a, kept)
+    _check(b[:, None], want["output"], "output")

@@ -422,3 +422,22 @@ def test_offsets_beyond_32_bits():
     net.updateGradInput([x, y], [x, y])
     for a, b in zip(net.gradInput, part.updateGradInput(tail, tail)):
         assert torch.equal(a[-64:], b)
+
+
+@pytest.mark.gpu
+def test_parameters_on_another_device_are_refused():
+    from fbcunn_amd import nn
+    x = torch.randn(2, 16, device="cuda")
+    with pytest.raises(ValueError, match="another device"):
+        nn.GatedResidualNorm(16, device="cpu").updateOutput([x, x, x])
+
+
+@pytest.mark.gpu
+def test_a_view_of_the_own_output_as_residual_keeps_its_values():
+    net = _net(48, "full", 1)
+    inputs, _ = _inputs((6, 48), "full", torch.float32, 6)
+    first = net.updateOutput(inputs)[0]
+    kept = first.clone()
+    again = net.updateOutput([first.view(6, 48), inputs[1], inputs[2]])
+    assert again[0] is not first and torch.equal(first, kept)
+    _check(again[1], _plain(net, [kept, inputs[1], inputs[2]])["normed"], "normed")
