@@ -188,6 +188,14 @@ __device__ __forceinline__ void step_four(const Four<P, G, BITS> &f, const Adamw
     }
 }
 
+// Counts one more of `all`; whether it is the last, which leaves the count at zero for the next step.
+__device__ __forceinline__ bool one_more(unsigned *count, unsigned all)
+{
+    if (__hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) != all - 1) return false;
+    __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+}
+
 template <typename P, typename G, int BITS>
 __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a)
 {
@@ -216,9 +224,11 @@ __global__ __launch_bounds__(256) void adamw_kernel(AdamwArgs a)
     // Every wavefront of this workgroup has read the clock; the last workgroup of all moves it on, so a step replayed
     // from a graph is the next step.
     __syncthreads();
-    if (threadIdx.x == 0 &&
-        __hip_atomic_fetch_add(&a.clock->done, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == gridDim.x - 1)
-        *a.clock = clock_of(now.t + 1, now.power1 * a.beta1, now.power2 * a.beta2, a.seed);
+    if (threadIdx.x == 0) {
+        const unsigned line = blockIdx.x % kAdamwLines, lines = min(gridDim.x, (unsigned)kAdamwLines);
+        if (one_more(a.ended + line * kAdamwLine, (gridDim.x - line + kAdamwLines - 1) / kAdamwLines) && one_more(&a.clock->done, lines))
+            *a.clock = clock_of(now.t + 1, now.power1 * a.beta1, now.power2 * a.beta2, a.seed);
+    }
 }
 
 hipError_t launch_adamw_set_clock(const AdamwArgs &a, long t, hipStream_t s)

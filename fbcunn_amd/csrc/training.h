@@ -25,12 +25,16 @@ struct AdamwClock {
     double inv_bias1;   // 1 / (1 - beta1^(t + 1))
     float inv_root2;    // 1 / sqrt(1 - beta2^(t + 1))
     unsigned key;       // of the random numbers of step t + 1
-    unsigned done;      // workgroups of the running step that have ended
+    unsigned done;      // lines of AdamwArgs::ended that are complete
 };
+// Workgroups of the running step that have ended, counted on lines of their own: additions to one address follow each
+// other 10 ns apart, and 2048 of them would take longer than a short step.
+constexpr int kAdamwLines = 32, kAdamwLine = 16;   // values of a line
 struct AdamwArgs {
     const AdamwPiece *pieces;
     int n_pieces;
     AdamwClock *clock;
+    unsigned *ended;   // kAdamwLines lines, all zero between steps
     void *m, *v;
     float *m_scale, *v_scale;
     double beta1, beta2;

@@ -6,6 +6,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
+#include <cstring>
 #include <new>
 #include <vector>
 
@@ -56,7 +57,7 @@ bool ranges_overlap(std::vector<Range> &r)
 struct fbfc_adamw {
     int device;
     fbfc_adamw_config config;
-    void *memory;  // the clock, then the table of pieces
+    void *memory;  // the clock, the counts of workgroups, the table of pieces
     fbfc::AdamwArgs args;
 };
 
@@ -145,12 +146,14 @@ static int adamw_create(const fbfc_adamw_config *c, const fbfc_adamw_tensor *ten
     fbfc_adamw *p = new (std::nothrow) fbfc_adamw();
     if (p == nullptr) return fail(FBFC_ERR_OUT_OF_MEMORY, "host allocation failed");
     p->config = *c;
-    constexpr size_t head = 256;
-    static_assert(sizeof(fbfc::AdamwClock) <= head, "the clock has a line of its own");
+    constexpr size_t counts = 256, head = counts + fbfc::kAdamwLines * fbfc::kAdamwLine * sizeof(unsigned);
+    static_assert(sizeof(fbfc::AdamwClock) <= counts, "the clock has a line of its own");
+    unsigned char begin[head] = {};
     const fbfc::AdamwClock clock = fbfc::adamw_clock(0, c->beta1, c->beta2, c->seed);
+    std::memcpy(begin, &clock, sizeof clock);
     hipError_t e = hipGetDevice(&p->device);
     if (e == hipSuccess) e = hipMalloc(&p->memory, head + pieces.size() * sizeof(fbfc::AdamwPiece));
-    if (e == hipSuccess) e = hipMemcpy(p->memory, &clock, sizeof clock, hipMemcpyHostToDevice);
+    if (e == hipSuccess) e = hipMemcpy(p->memory, begin, sizeof begin, hipMemcpyHostToDevice);
     if (e == hipSuccess && !pieces.empty())
         e = hipMemcpy(static_cast<char *>(p->memory) + head, pieces.data(), pieces.size() * sizeof(fbfc::AdamwPiece),
                       hipMemcpyHostToDevice);
@@ -164,6 +167,7 @@ static int adamw_create(const fbfc_adamw_config *c, const fbfc_adamw_tensor *ten
     a.pieces = reinterpret_cast<const fbfc::AdamwPiece *>(static_cast<char *>(p->memory) + head);
     a.n_pieces = (int)pieces.size();
     a.clock = static_cast<fbfc::AdamwClock *>(p->memory);
+    a.ended = reinterpret_cast<unsigned *>(static_cast<char *>(p->memory) + counts);
     a.m = m;
     a.v = v;
     a.m_scale = m_scale;
