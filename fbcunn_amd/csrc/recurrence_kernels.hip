@@ -42,7 +42,8 @@ constexpr int kLanes = 64;
 // tiles 31 and 10), or, with half of the CUs at work anyway, 5 (128 columns in bf16: 3 tiles 14.9 and 17.5, 4 tiles
 // 20.3 and 19.8, 12 tiles 54 and 39).
 constexpr int kGroups = 256;
-constexpr int kHead = 256;    // bytes of the workspace before the announcements
+constexpr int kCounters = 8, kCounterLine = 32, kFew = 1024;  // see draw()
+constexpr int kHead = kCounters * kCounterLine * (int)sizeof(unsigned);  // bytes of the workspace before the announcements
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Announcements.  A word is announced once it differs from what the workspace is filled with, all ones (a NaN that
@@ -54,7 +55,7 @@ constexpr word64 kUnset2 = ~0ull;
 __device__ __forceinline__ unsigned announced(float v) { return v != v ? 0x7FC00000u : __float_as_uint(v); }
 
 struct Chain {
-    unsigned *ticket;   // of the next tile to be given out, less one
+    unsigned *tickets;  // of the next tile that each counter gives out, less one
     word64 *runs;       // (A, S) of each tile and channel
     unsigned *states;   // the state behind each tile
 };
@@ -82,7 +83,7 @@ __host__ __device__ __forceinline__ Shape shape_of(int batch, int channels, long
 __device__ __forceinline__ Chain chain_of(unsigned char *workspace, const Shape &s, int v)
 {
     Chain c;
-    c.ticket = reinterpret_cast<unsigned *>(workspace);
+    c.tickets = reinterpret_cast<unsigned *>(workspace);
     c.runs = reinterpret_cast<word64 *>(workspace + kHead);
     c.states = reinterpret_cast<unsigned *>(c.runs + (long)s.tiles * s.cols * kLanes * v);
     return c;
@@ -270,9 +271,18 @@ __device__ __forceinline__ float closed(float gate, float bias2, float &e)
 // other, those of different columns side by side: what is worked on at one time lies in the same rows of memory.  Other ways
 // of giving out tiles, on the forward pass over 131072 steps of 2048 channels in bf16 (385 us so): a counter for each column, 399
 // us; that with the columns kept to one XCD, 454 us; workgroups that stay and draw their next tile ahead, 417 us.
-__device__ __forceinline__ unsigned draw(const Chain &ch)
+//
+// Additions to one address follow each other about 10 ns apart, which the first 512 workgroups of a launch wait for.  Where
+// there are few more than these, 8 counters give out the tiles of every eighth column each (5 sequences of 1537 steps x 515
+// channels in 32 bits: 585 workgroups, a training step 50.1 us with one counter, 45.6 so).  Where there are many, columns that
+// drift apart cost more than the start (32 counters on the 49152 of the long sequence above: 1163 us, one 1049).
+__device__ __forceinline__ unsigned draw(const Chain &ch, const Shape &s)
 {
-    return __hip_atomic_fetch_add(ch.ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+    const unsigned cols = s.cols, few = s.tiles * s.cols <= kFew, counter = few ? blockIdx.x % cols % kCounters : 0;
+    const unsigned n = __hip_atomic_fetch_add(ch.tickets + counter * kCounterLine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
+    if (!few) return n;
+    const unsigned columns = (cols - counter + kCounters - 1) / kCounters;
+    return n / columns * cols + n % columns * kCounters + counter;
 }
 __device__ __forceinline__ long length_of(const int *lengths, int b, long steps)
 {
@@ -343,7 +353,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
     unsigned long ticket = blockIdx.x;
     const unsigned long all = (unsigned long)s.tiles * s.cols;
     if (s.chain) {
-        if (threadIdx.x == 0) given = draw(ch);
+        if (threadIdx.x == 0) given = draw(ch, s);
         __syncthreads();
         ticket = __builtin_amdgcn_readfirstlane(given);
     }
@@ -467,7 +477,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
     unsigned long ticket = blockIdx.x;
     const unsigned long all = (unsigned long)s.tiles * s.cols;
     if (s.chain) {
-        if (threadIdx.x == 0) given = draw(ch);
+        if (threadIdx.x == 0) given = draw(ch, s);
         __syncthreads();
         ticket = __builtin_amdgcn_readfirstlane(given);
     }
