@@ -6,7 +6,7 @@ import torch
 
 from . import _lib
 from ._lib import RecurrenceDesc, ResidualNormDesc, Rows, Steps, check, lib
-from .tensors import TYPES, Workspace, _ptr, _stream, check_current, signature
+from .tensors import TYPES, Workspace, _ptr, signature, stream_on
 
 __all__ = ["GatedLinearRecurrence", "GatedResidualNorm"]
 
@@ -30,37 +30,66 @@ def _check_device(t, parameters):
         raise ValueError("the inputs are on another device than the parameters")
 
 
-def _like(old, t):
-    """`old` where it can take what has the shape and the type of t, else a new tensor."""
-    if old is not None and old.shape == t.shape and old.dtype == t.dtype and old.device == t.device:
-        return old
-    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
+class _Call:
+    """What a module's calls on inputs of one signature share, and the results that it makes for them."""
+
+    def __init__(self, like, results):
+        self.shape, self.dtype, self.device, self.index = like.shape, like.dtype, like.device, like.device.index
+        self.bytes = like.numel() * like.element_size()
+        self.captured = False
+        self._made = [(None, 0)] * results
+
+    def result(self, i, places=()):
+        """Result i, the tensor of the last call unless one of `places` lies in it: an input that is a module's last
+        output, or a view of it, keeps its values, which backward reads."""
+        t, at = self._made[i]
+        if t is not None:
+            for p in places:
+                if at <= p < at + self.bytes:
+                    break
+            else:
+                return t
+        return self._make(i, self.shape, self.dtype)
+
+    def _make(self, i, shape, dtype):
+        t = torch.empty(shape, dtype=dtype, device=self.device)
+        self._made[i] = t, t.data_ptr()
+        return t
 
 
-def _apart(old, inputs):
-    """`old`, or None where one of the inputs lies in it: an input that is a module's last output, or a view of it, keeps
-    its values, which backward reads."""
-    if old is None:
-        return None
-    at = old.data_ptr()
-    end = at + old.nbytes
-    for t in inputs:
-        if at <= t.data_ptr() < end:
-            return None
-    return old
+class _Calls:
+    """A module's call for the inputs that it was last given.  One that a graph was captured from is kept with its results,
+    which the graph writes to whenever it is replayed."""
+
+    def __init__(self, kind, *more):
+        self._kind, self._more, self._signature, self._call, self._captured = kind, more, None, None, []
+
+    def of(self, net, inputs):
+        now = signature(*inputs)
+        if now != self._signature:
+            call = self._kind(net, inputs, *self._more)
+            if self._call is not None and self._call.captured:
+                self._captured.append(self._call)
+            self._call, self._signature = call, now
+        call = self._call
+        if torch.cuda.is_current_stream_capturing():
+            call.captured = True
+        return call
 
 
-class _RecurrenceCall:
-    """What calls of the recurrence on inputs of one signature share: checked sizes and descriptors."""
+class _RecurrenceCall(_Call):
+    """Of the recurrence: checked sizes and descriptors.  Results: the output, the gradients of x and gate, the last state and the
+    gradient of the first."""
 
-    def __init__(self, net, x, gate, dims):
+    def __init__(self, net, input, dims):
+        x, gate = input
         channels = net.nChannels
         _check_activation(x, "x")
         _check_activation(gate, "gate", x)
         if x.dim() != dims or x.size(-1) != channels:
             raise ValueError("x must be (%s%d)" % ("batch, steps, " if dims == 3 else "batch, ", channels))
-        self.shape, self.dtype, self.device, self.index = x.shape, x.dtype, x.device, x.device.index
         _check_device(x, net.parameters())
+        super().__init__(x, 5)
         self.batch, steps = x.size(0), x.size(1) if dims == 3 else 1
         desc = RecurrenceDesc(self.batch, channels, steps, TYPES[x.dtype])
         self.desc = ctypes.byref(desc)
@@ -71,6 +100,10 @@ class _RecurrenceCall:
         # x, gate, output, gradients of x and gate, gradient of the output (its strides are those of each call)
         self.steps = [Steps(0, *s) for s in (strides[0], strides[1], whole, whole, whole, whole)]
         self.refs = [ctypes.byref(s) for s in self.steps]
+
+    def state(self, i):
+        t = self._made[i][0]
+        return self._make(i, (self.batch, self.shape[-1]), torch.float32) if t is None else t
 
 
 class GatedLinearRecurrence:
@@ -95,7 +128,7 @@ class GatedLinearRecurrence:
         self.train = True
         self.output = self.state = self.gradInput = self.gradState = None
         self._workspace, self._checkpoints = Workspace(), Workspace()
-        self._calls = {2: (None, None), 3: (None, None)}   # the last signature of step and updateOutput, and its call
+        self._calls = {dims: _Calls(_RecurrenceCall, dims) for dims in (2, 3)}   # of step and updateOutput
         self._forward = None   # (shape, type, lengths, checkpoints) of the updateOutput that backward may follow
 
     def training(self):
@@ -113,15 +146,10 @@ class GatedLinearRecurrence:
     def _call(self, input, dims):
         if len(input) != 2:
             raise ValueError("the input is [x, gate]")
-        x, gate = input
-        of = signature(x, gate)
-        last, call = self._calls[dims]
-        if last != of:
-            call = _RecurrenceCall(self, x, gate, dims)
-            self._calls[dims] = (of, call)
-        check_current(call.index)
-        call.steps[0].data, call.steps[1].data = x.data_ptr(), gate.data_ptr()
-        return call
+        call = self._calls[dims].of(self, input)
+        places = input[0].data_ptr(), input[1].data_ptr()
+        call.steps[0].data, call.steps[1].data = places
+        return call, places, stream_on(call.index)
 
     def _check_state(self, t, name, call):
         if t is None:
@@ -146,22 +174,17 @@ class GatedLinearRecurrence:
             raise ValueError("lengths must be %d contiguous numbers on the inputs' device" % call.batch)
         return t.data_ptr()
 
-    def _state_like(self, old, call):
-        if old is not None and old.size(0) == call.batch and old.device == call.device:
-            return old
-        return torch.empty(call.batch, self.nChannels, device=call.device)
-
     def updateOutput(self, input, state=None, lengths=None):
-        call = self._call(input, 3)
+        call, places, stream = self._call(input, 3)
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
-        self.output = _like(_apart(self.output, input), call)
-        self.state = self._state_like(self.state, call)
+        self.output = call.result(0, places)
+        self.state = call.state(3)
         kept = self._checkpoints.take(call.checkpointBytes, call.device) if self.train else None
         call.steps[2].data = self.output.data_ptr()
         self._forward = None
         check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), first, sizes, call.refs[2],
                                             self.state.data_ptr(), kept.data_ptr() if self.train else None,
-                                            self._workspace.take(call.workspaceBytes, call.device).data_ptr(), _stream()))
+                                            self._workspace.take(call.workspaceBytes, call.device).data_ptr(), stream))
         if self.train:
             self._forward = (call.shape, call.dtype, lengths, kept)
         return self.output
@@ -170,18 +193,18 @@ class GatedLinearRecurrence:
 
     def step(self, input, state):
         """One token of each sequence: [x, gate] of (batch, nChannels); advances `state` in place and gives the output."""
-        call = self._call(input, 2)
+        call, places, stream = self._call(input, 2)
         if state is None:
             raise TypeError("step needs the state that it advances")
         at = self._check_state(state, "state", call)
-        self.output = _like(_apart(self.output, input), call)
+        self.output = call.result(0, places)
         call.steps[2].data = self.output.data_ptr()
         check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), at, None, call.refs[2], at, None,
-                                            None, _stream()))
+                                            None, stream))
         return self.output
 
     def _backward(self, input, gradOutput, gradState, inputs, weights, scale):
-        call = self._call(input, 3)
+        call, _, stream = self._call(input, 3)
         shape, dtype, lengths, kept = self._forward or (None, None, None, None)
         if shape != call.shape or dtype != call.dtype or kept.device != call.device:
             raise ValueError("backward follows an updateOutput of the same inputs, not after evaluate()")
@@ -192,16 +215,15 @@ class GatedLinearRecurrence:
         of.stride_batch, of.stride_step, of.stride_channel = gradOutput.stride()
         grads, first = (None, None), None
         if inputs:
-            old = self.gradInput or (None, None)
-            self.gradInput = [_like(old[0], call), _like(old[1], call)]
+            self.gradInput = [call.result(1), call.result(2)]
             call.steps[3].data, call.steps[4].data = (t.data_ptr() for t in self.gradInput)
             grads = call.refs[3:5]
-            self.gradState = self._state_like(self.gradState, call)
+            self.gradState = call.state(4)
             first = self.gradState.data_ptr()
         check(lib().fbfc_recurrence_backward(call.desc, *call.refs[:2], self.bias.data_ptr(), _ptr(lengths), kept.data_ptr(),
                                              call.refs[5], last, *grads,
                                              self.gradBias.data_ptr() if weights else None, scale, first,
-                                             self._workspace.take(call.workspaceBytes, call.device).data_ptr(), _stream()))
+                                             self._workspace.take(call.workspaceBytes, call.device).data_ptr(), stream))
 
     def updateGradInput(self, input, gradOutput, gradState=None):
         """[gradient of x, gradient of gate]; self.gradState is the gradient of the state before the first step.  `gradState`:
@@ -218,8 +240,8 @@ class GatedLinearRecurrence:
         return self.gradInput
 
 
-class _NormCall:
-    """What calls of the norms on inputs of one signature share: checked sizes and descriptors."""
+class _NormCall(_Call):
+    """Of the norms: checked sizes and descriptors.  Results: output, normed, the gradients of the inputs."""
 
     def __init__(self, net, input):
         residual = input[0]
@@ -229,7 +251,7 @@ class _NormCall:
         for t, name in zip(input[1:], net._names[1:]):
             _check_activation(t, name, residual)
         _check_device(residual, net.parameters())
-        self.shape, self.dtype, self.device, self.index = residual.shape, residual.dtype, residual.device, residual.device.index
+        super().__init__(residual, 2 + len(input))
         self.sizes = ResidualNormDesc(residual.numel() // net.nChannels, net.nChannels, TYPES[residual.dtype], net.eps)
         self.desc = ctypes.byref(self.sizes)
         self.workspaceBytes = lib().fbfc_residual_norm_workspace_bytes(self.desc)
@@ -275,7 +297,7 @@ class GatedResidualNorm:
         self.output, self.gradInput = None, None
         self._workspace = Workspace()
         self._names = ("residual", "branch", "gate")[:1 + self.hasBranch + self.hasGate]
-        self._signature = self._last = None   # of the last inputs, and what their calls share
+        self._calls = _Calls(_NormCall)
 
     def parameters(self):
         pairs = [(self.postWeight, self.gradPostWeight), (self.scale, self.gradScale), (self.preWeight, self.gradPreWeight)]
@@ -302,24 +324,19 @@ class GatedResidualNorm:
             input = [input]
         if len(input) != len(self._names):
             raise ValueError("the input is [%s]" % ", ".join(self._names))
-        of = signature(*input)
-        if of != self._signature:
-            self._last, self._signature = _NormCall(self, input), of
-        call = self._last
-        check_current(call.index)
+        call = self._calls.of(self, input)
         call.sizes.eps = self.eps
-        for rows, t in zip(call.rows, input):
-            rows.data = t.data_ptr()
-        return call, input
+        places = [t.data_ptr() for t in input]
+        for rows, p in zip(call.rows, places):
+            rows.data = p
+        return call, input, places, stream_on(call.index)
 
     def updateOutput(self, input):
-        call, input = self._call(input)
-        # without a branch the first output is the caller's tensor, never one to write into
-        old = [_apart(t, input) for t in self.output or (None, None)]
-        output = _like(old[0], call) if self.hasBranch else None
-        normed = _like(old[1], call) if self.hasNorm else None
+        call, input, places, stream = self._call(input)
+        output = call.result(0, places) if self.hasBranch else None
+        normed = call.result(1, places) if self.hasNorm else None
         check(lib().fbfc_residual_norm_forward(call.desc, *call.inputs, *self._weights(), call.at(3, output), call.at(4, normed),
-                                               _stream()))
+                                               stream))
         self.output = [output if self.hasBranch else input[0], normed]
         return self.output
 
@@ -329,7 +346,7 @@ class GatedResidualNorm:
         return [None if t is None else t.data_ptr() for t in (self.postWeight, self.scale, self.preWeight)]
 
     def _backward(self, input, gradOutput, inputs, weights, scale):
-        call, input = self._call(input)
+        call, input, _, stream = self._call(input)
         gr, gn = gradOutput
         if gr is None and gn is None:
             raise ValueError("gradOutput is [gradOutput, gradNormed], and one of them is needed")
@@ -341,15 +358,14 @@ class GatedResidualNorm:
                 call.rows[i].stride = self._row_stride(t, name)
         grads = [None] * 3
         if inputs:
-            old = self.gradInput or [None] * 3
-            self.gradInput = [_like(old[i], call) for i in range(len(input))]
+            self.gradInput = [call.result(2 + i) for i in range(len(input))]
             grads[:len(input)] = [call.at(7 + i, t) for i, t in enumerate(self.gradInput)]
         ws, params = None, [None] * 3
         if weights:
             ws = self._workspace.take(call.workspaceBytes, call.device).data_ptr()
             params = [None if t is None else t.data_ptr() for t in (self.gradPostWeight, self.gradScale, self.gradPreWeight)]
         check(lib().fbfc_residual_norm_backward(call.desc, *call.inputs, *self._weights(), call.at(5, gr), call.at(6, gn), *grads,
-                                                *params, scale, ws, _stream()))
+                                                *params, scale, ws, stream))
 
     def updateGradInput(self, input, gradOutput):
         self._backward(input, gradOutput, True, False, 1.0)

@@ -25,9 +25,11 @@ def signature(*tensors):
         raise TypeError("CUDA tensors are needed") from None
 
 
-def check_current(index):
-    if torch.cuda.current_device() != index:
+def stream_on(index):
+    """The current stream, if device `index` is the current one."""
+    if torch._C._cuda_getDevice() != index:
         raise ValueError("the tensors are not on the current device")
+    return torch._C._cuda_getCurrentRawStream(index)
 
 
 def _check_tensor(t, name, ndim=None, strided=False):

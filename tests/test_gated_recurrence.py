@@ -506,3 +506,31 @@ def test_views_of_the_own_output_as_input_keep_their_values():
     want = _plain(kept[:, None], kept[:, None], net.bias, None, None, kept[:, None], None)
     assert b is not a and torch.equal(a, kept)
     _check(b[:, None], want["output"], "output")
+
+
+@pytest.mark.gpu
+def test_a_graph_keeps_its_results_when_the_module_goes_on_with_other_shapes():
+    net, x, gate, gy, h0, gh = _data(2, 150, 40, torch.float32, 19)
+    other, *_ = _data(2, 150, 40, torch.float32, 19)
+
+    def step(m, n=150):
+        m.updateOutput([x[:, :n], gate[:, :n]], state=h0)
+        m.backward([x[:, :n], gate[:, :n]], gy[:, :n], gradState=gh)
+
+    step(net)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(net)
+    y = net.output
+    for n in (70, 150, 3):
+        step(net, n)
+    # memory that the module has given back would be found here
+    fill = [torch.full((k,), 7.0, device="cuda") for k in (80, 2 * 150 * 40) for _ in range(20)]
+    for rep in range(3):
+        x.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(bool((t == 7.0).all()) for t in fill)
+        step(other)
+        assert torch.equal(y, other.output) and torch.equal(net.gradBias, other.gradBias)

@@ -441,3 +441,31 @@ def test_a_view_of_the_own_output_as_residual_keeps_its_values():
     again = net.updateOutput([first.view(6, 48), inputs[1], inputs[2]])
     assert again[0] is not first and torch.equal(first, kept)
     _check(again[1], _plain(net, [kept, inputs[1], inputs[2]])["normed"], "normed")
+
+
+@pytest.mark.gpu
+def test_a_graph_keeps_its_results_when_the_module_goes_on_with_other_shapes():
+    net, other = _net(40, "full", 1), _net(40, "full", 1)
+    inputs, grads = _inputs((70, 40), "full", torch.float32, 7)
+
+    def step(m, n=70):
+        m.updateOutput([t[:n] for t in inputs])
+        m.backward([t[:n] for t in inputs], [t[:n] for t in grads])
+
+    step(net)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(net)
+    out, normed = net.output
+    for n in (30, 70, 1):
+        step(net, n)
+    fill = [torch.full((70 * 40,), 7.0, device="cuda") for _ in range(20)]   # memory that the module has given back would be found here
+    for rep in range(3):
+        inputs[0].mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(bool((t == 7.0).all()) for t in fill)
+        step(other)
+        assert torch.equal(out, other.output[0]) and torch.equal(normed, other.output[1])
+        assert torch.equal(net.gradScale, other.gradScale)
