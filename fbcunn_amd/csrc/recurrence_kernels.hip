@@ -42,8 +42,8 @@ constexpr int kLanes = 64;
 // tiles 31 and 10), or, with half of the CUs at work anyway, 5 (128 columns in bf16: 3 tiles 14.9 and 17.5, 4 tiles
 // 20.3 and 19.8, 12 tiles 54 and 39).
 constexpr int kGroups = 256;
-constexpr int kCounters = 8, kCounterLine = 32, kFew = 1024;  // see draw()
-constexpr int kHead = kCounters * kCounterLine * (int)sizeof(unsigned);  // bytes of the workspace before the announcements
+constexpr int kXcds = 8, kCounterLine = 32, kFew = 2048;  // see draw()
+constexpr int kHead = kXcds * kCounterLine * (int)sizeof(unsigned);  // bytes of the workspace before the announcements
 constexpr float kLog2e = 1.44269504088896340736f;
 
 // Announcements.  A word is announced once it differs from what the workspace is filled with, all ones (a NaN that
@@ -273,16 +273,27 @@ __device__ __forceinline__ float closed(float gate, float bias2, float &e)
 // us; that with the columns kept to one XCD, 454 us; workgroups that stay and draw their next tile ahead, 417 us.
 //
 // Additions to one address follow each other about 10 ns apart, which the first 512 workgroups of a launch wait for.  Where
-// there are few more than these, 8 counters give out the tiles of every eighth column each (5 sequences of 1537 steps x 515
-// channels in 32 bits: 585 workgroups, a training step 50.1 us with one counter, 45.6 so).  Where there are many, columns that
-// drift apart cost more than the start (32 counters on the 49152 of the long sequence above: 1163 us, one 1049).
+// there are few, 8 counters give out the tiles of an eighth of the columns each (5 sequences of 1537 steps x 515
+// channels in 32 bits: 585 workgroups, a training step 50.1 us with one counter, 45.6 so; 4 x 3219 x 714 in fp16, up to
+// 1248: 75 and 65).  Where there are many, columns that drift apart cost more than the start (a training step of 1 x 30000 x
+// 2048 in bf16, up to 7520: 264 us with one counter, 274 with 8; of the long sequence above, 32768: 1049 and 1139).
+//
+// Workgroups go to the 8 XCDs in turn, so every eighth one takes columns beside each other: where rows do not begin on a line
+// of memory, two columns share lines, which one L2 cache then reads and writes once (64 sequences of 128 steps x 1001
+// channels in 32 bits: a training step 84 us with columns in turn, 69 so; 37 x 287 x 1723 171 and 149, with 1728 channels 131 and
+// 134).
+__device__ __forceinline__ unsigned column_of(unsigned i, unsigned cols)
+{
+    const unsigned xcd = i % kXcds, more = cols % kXcds;
+    return xcd * (cols / kXcds) + (xcd < more ? xcd : more) + i / kXcds;
+}
 __device__ __forceinline__ unsigned draw(const Chain &ch, const Shape &s)
 {
-    const unsigned cols = s.cols, few = s.tiles * s.cols <= kFew, counter = few ? blockIdx.x % cols % kCounters : 0;
+    const unsigned cols = s.cols, few = s.tiles * s.cols <= kFew, counter = few ? blockIdx.x % cols % kXcds : 0;
     const unsigned n = __hip_atomic_fetch_add(ch.tickets + counter * kCounterLine, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) + 1u;
     if (!few) return n;
-    const unsigned columns = (cols - counter + kCounters - 1) / kCounters;
-    return n / columns * cols + n % columns * kCounters + counter;
+    const unsigned columns = (cols - counter + kXcds - 1) / kXcds;
+    return n / columns * cols + column_of(n % columns * kXcds + counter, cols);
 }
 __device__ __forceinline__ long length_of(const int *lengths, int b, long steps)
 {
@@ -350,7 +361,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
     const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    unsigned long ticket = blockIdx.x;
+    unsigned long ticket = s.chain ? 0 : column_of(blockIdx.x, s.cols);
     const unsigned long all = (unsigned long)s.tiles * s.cols;
     if (s.chain) {
         if (threadIdx.x == 0) given = draw(ch, s);
@@ -474,7 +485,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
     const Shape s = shape_of(a.batch, a.channels, steps, V);
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const Chain ch = chain_of(a.workspace, s, V);
-    unsigned long ticket = blockIdx.x;
+    unsigned long ticket = s.chain ? 0 : column_of(blockIdx.x, s.cols);
     const unsigned long all = (unsigned long)s.tiles * s.cols;
     if (s.chain) {
         if (threadIdx.x == 0) given = draw(ch, s);
