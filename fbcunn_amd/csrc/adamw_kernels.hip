@@ -21,7 +21,8 @@
 // gradients and 8-bit states 726 us (4.84 TB/s); 25 million in bf16 with 8-bit states, unaligned, 62 us (4.06 TB/s; here
 // the arithmetic of the rounding counts, with divisions and roots rounded to half a unit 69 us).  Non-temporal stores,
 // 1024 to 4096 workgroups and 8 or 16 parameters in flight a lane are all within 3 %; a workgroup for each piece is
-// slower with 8-bit states (783 us).
+// slower with 8-bit states (783 us).  2.9 million of 126 tensors: 13.2 us with 8-bit states, 16.7 in 32 bits (30.7 and 32.7
+// where all workgroups report their end at one address).
 #include <hip/hip_runtime.h>
 
 #include <cmath>
