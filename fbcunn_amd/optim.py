@@ -21,7 +21,8 @@ class AdamW:
     written into them before each step, as the modules' accGradParameters does.  With stateBits = 32 the states `m` and
     `v` are float32, with 8 they are float8_e4m3fn with a float32 scale per 256 elements (`mScale`, `vScale`), rounded
     at random (from `seed` and the number of the step).  In the states every tensor begins at a multiple of 256 elements.
-    `lr` and `weightDecay` may be changed between steps.  A step captured into a graph is a new step at each replay."""
+    `lr` and `weightDecay` may be changed between steps.  A step captured into a graph is a new step at each replay,
+    for as long as the optimizer lives."""
 
     def __init__(self, params, grads, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weightDecay=1e-2, stateBits=32, seed=0):
         self._handle = ctypes.c_void_p(0)

@@ -534,3 +534,22 @@ def test_a_graph_keeps_its_results_when_the_module_goes_on_with_other_shapes():
         assert all(bool((t == 7.0).all()) for t in fill)
         step(other)
         assert torch.equal(y, other.output) and torch.equal(net.gradBias, other.gradBias)
+
+
+@pytest.mark.gpu
+def test_a_captured_step_is_a_new_token_at_each_replay():
+    net, x, gate, _, h0, _ = _data(5, 7, 70, torch.bfloat16, 20)
+    other, *_ = _data(5, 7, 70, torch.bfloat16, 20)
+    state, want = h0.clone(), h0.clone()
+    at, to = x[:, 0].clone(), gate[:, 0].clone()
+    net.step([at, to], state.clone())
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = net.step([at, to], state)
+    for t in range(7):
+        at.copy_(x[:, t])
+        to.copy_(gate[:, t])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, other.step([x[:, t], gate[:, t]], want)) and torch.equal(state, want)
