@@ -183,18 +183,22 @@ __device__ __forceinline__ void announce_state(const Chain &ch, const Shape &s, 
 
 // A tensor's rows as a lane reads and writes them: V channels from c on.  Where the last block of channels ends inside
 // or before a lane, its loads are moved back to end with the row, so that no load has a condition, and an odd last channel
-// is then moved to its place.  DENSE: channels side by side, with an offset that fits 32 bits, so that the row's
-// address stays in scalar registers.
+// is then moved to its place.  Orders of memory: kDense, channels side by side, with an offset that fits 32 bits, so that the
+// row's address stays in scalar registers; kPlanes, steps side by side, as a convolution leaves them: each lane reads its 16
+// steps in vectors of 16 bytes (8 sequences of 2048 steps x 1024 channels in 32 bits, input and gate in planes, forward 42 us so, 76
+// one step at a time; 38 with the channels side by side; in bf16 28.5, 77 and 28); kAny.
 //
 // Forward, a lane has 4 bytes of each row, two channels in 16 bits.  Backward it has one: with two, a wavefront needs 178
 // registers instead of 111, and one workgroup fits a CU where two do (131072 steps of 2048 channels in bf16: 752 us with two
 // channels, 662 with one; forward 393 with two and 425 with one).
-template <typename T, bool DENSE>
-constexpr int kLaneChannels = DENSE && sizeof(T) == 2 ? 2 : 1;
+enum Order { kAny, kDense, kPlanes };
+template <typename T, Order IN>
+constexpr int kLaneChannels = IN == kDense && sizeof(T) == 2 ? 2 : 1;
+constexpr Order kOut(Order in) { return in == kAny ? kAny : kDense; }  // of what is written
 
-template <typename T, bool DENSE, int V>
+template <typename T, Order ORDER, int V>
 struct LaneRows {
-    typedef typename std::conditional<DENSE, unsigned, long>::type Offset;
+    typedef typename std::conditional<ORDER == kDense, unsigned, long>::type Offset;
     const char *base;
     long st;             // bytes from row to row
     Offset off;          // of this lane's loads in a row, in bytes
@@ -203,7 +207,7 @@ struct LaneRows {
         base = static_cast<const char *>(t.data) + (long)b * t.sb * (long)sizeof(T);
         st = t.st * (long)sizeof(T);
         const int first = c + V <= channels ? c : channels - V;
-        off = (Offset)(DENSE ? (long)first * (long)sizeof(T) : first * t.sc * (long)sizeof(T));
+        off = (Offset)(ORDER == kDense ? (long)first * (long)sizeof(T) : first * t.sc * (long)sizeof(T));
     }
     __device__ __forceinline__ const char *row(long step) const
     {
@@ -216,7 +220,7 @@ struct LaneRows {
     __device__ __forceinline__ T *place(const char *row) const
     {
         Offset o = off;
-        if constexpr (DENSE) asm("" : "+s"(row), "+v"(o));
+        if constexpr (ORDER == kDense) asm("" : "+s"(row), "+v"(o));
         return reinterpret_cast<T *>(const_cast<char *>(row) + o);
     }
     // 16 rows from step t0 on, of which `n` are the sequence's; the others repeat its last one (there is one).  FULL: all are
@@ -225,6 +229,19 @@ struct LaneRows {
     __device__ __forceinline__ void load(Vec<T, V> (&v)[kRun], long t0, int n, long len, int c, int channels) const
     {
         const char *r = row(FULL || n > 0 ? t0 : len - 1);
+        if constexpr (ORDER == kPlanes) {
+            static_assert(V == 1, "a lane walks along one line");
+            if (FULL || n == kRun) {
+                constexpr int N = 16 / (int)sizeof(T);
+                const T *p = place(r);
+                Vec<T, N> w[kRun / N];
+#pragma unroll
+                for (int j = 0; j < kRun / N; ++j) w[j] = load_vec<N>(p + j * N);
+#pragma unroll
+                for (int t = 0; t < kRun; ++t) v[t][0] = w[t / N][t % N];
+                return;
+            }
+        }
 #pragma unroll
         for (int t = 0; t < kRun; ++t) {
             v[t] = load_vec<V>(place(r));
@@ -351,10 +368,10 @@ __device__ __forceinline__ void fill_runs(float (*to)[kWaves][kLanes * V], int w
         for (int i = threadIdx.x; i < kLanes * V; i += blockDim.x) to[0][j][i] = to[1][j][i] = v;
 }
 
-template <typename T, bool DENSE>
+template <typename T, Order IN>
 __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(RecArgs a)
 {
-    constexpr int V = kLaneChannels<T, DENSE>;
+    constexpr int V = kLaneChannels<T, IN>;
     __shared__ float sA[2][kWaves][kLanes * V], sS[2][kWaves][kLanes * V], carried[kLanes * V];
     __shared__ unsigned given;
     const long steps = a.steps;
@@ -375,7 +392,8 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
         const int order = (int)(ticket / (unsigned)s.cols), col = (int)(ticket % (unsigned)s.cols), tile = order;
         const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
         const long len = length_of(a.lengths, b, steps);
-        const LaneRows<T, DENSE, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels);
+        const LaneRows<T, IN, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels);
+        const LaneRows<T, kOut(IN), V> yr(a.y, b, c, a.channels);
         const bool whole = __all(c + V <= a.channels);
         float bias2[V];
 #pragma unroll
@@ -475,7 +493,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
     }
 }
 
-template <typename T, bool DENSE>
+template <typename T, Order IN, Order GRAD>
 __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(RecArgs a, float *partial)
 {
     constexpr int V = 1;
@@ -500,8 +518,9 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
         const int order = (int)(ticket / (unsigned)s.cols), col = (int)(ticket % (unsigned)s.cols), tile = s.tiles - 1 - order;
         const int b = col / s.blocks, c = col % s.blocks * kLanes * V + lane * V;
         const long len = length_of(a.lengths, b, steps);
-        const LaneRows<T, DENSE, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels), yr(a.y, b, c, a.channels),
-            gxr(a.grad_x, b, c, a.channels), ggr(a.grad_gate, b, c, a.channels);
+        const LaneRows<T, IN, V> xr(a.x, b, c, a.channels), gr(a.gate, b, c, a.channels);
+        const LaneRows<T, GRAD, V> yr(a.y, b, c, a.channels);
+        const LaneRows<T, kOut(IN), V> gxr(a.grad_x, b, c, a.channels), ggr(a.grad_gate, b, c, a.channels);
         const bool whole = __all(c + V <= a.channels);
         float bias2[V];
 #pragma unroll
@@ -719,14 +738,13 @@ static hipError_t launch_bias(const float *partial, long rows, const RecArgs &a,
     return hipGetLastError();
 }
 
-// Whether the channels of every tensor lie side by side, in rows that 32 bits reach over.
-static bool dense(int type, const RecArgs &a)
+// The order of a tensor's memory; rows of dense ones are within the reach of 32 bits.
+static Order order_of(int type, const Steps &t, const RecArgs &a)
 {
-    if (a.channels < (type == kF32 ? 1 : 2) || a.channels > 1 << 29) return false;
-    for (const Steps *t : {&a.x, &a.gate, &a.y, &a.grad_x, &a.grad_gate})
-        if (t->data != nullptr && t->sc != 1) return false;
-    return true;
+    if (t.sc == 1 && a.channels >= (type == kF32 ? 1 : 2) && a.channels <= 1 << 29) return kDense;
+    return t.st == 1 ? kPlanes : kAny;
 }
+static bool dense(int type, const Steps &t, const RecArgs &a) { return t.data == nullptr || order_of(type, t, a) == kDense; }
 
 size_t recurrence_checkpoint_bytes(int batch, int channels, long steps)
 {
@@ -770,10 +788,11 @@ static hipError_t clear_chain(const RecArgs &a, const Shape &s, int v, hipStream
 template <typename T>
 static hipError_t forward_typed(int type, const RecArgs &a, hipStream_t stream)
 {
-    const bool side = dense(type, a);
-    const int v = side ? kLaneChannels<T, true> : 1;
+    const bool out = dense(type, a.y, a);
+    const Order x = order_of(type, a.x, a), in = out && x == order_of(type, a.gate, a) ? x : kAny;
+    const int v = in == kDense ? kLaneChannels<T, kDense> : 1;
     if (a.steps <= 1) {
-        const bool wide = side && a.channels >= 4;
+        const bool wide = in == kDense && a.channels >= 4;
         const long lanes = (long)a.batch * ((a.channels + (wide ? 3 : 0)) / (wide ? 4 : 1));
         const dim3 grid((unsigned)((lanes + 255) / 256));
         kernel_log_add("recurrence_step_kernel", (long)grid.x * 256);
@@ -788,15 +807,18 @@ static hipError_t forward_typed(int type, const RecArgs &a, hipStream_t stream)
     }
     const dim3 grid(s.chain ? s.tiles * s.cols : s.cols), block(s.waves * kLanes);
     kernel_log_add(s.chain ? "recurrence_forward_kernel<chain>" : "recurrence_forward_kernel", (long)grid.x * block.x);
-    if (side) FBFC_LAUNCH((recurrence_forward_kernel<T, true>), grid, block, 0, stream, a);
-    else FBFC_LAUNCH((recurrence_forward_kernel<T, false>), grid, block, 0, stream, a);
+    if (in == kDense) FBFC_LAUNCH((recurrence_forward_kernel<T, kDense>), grid, block, 0, stream, a);
+    else if (in == kPlanes) FBFC_LAUNCH((recurrence_forward_kernel<T, kPlanes>), grid, block, 0, stream, a);
+    else FBFC_LAUNCH((recurrence_forward_kernel<T, kAny>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
 
 template <typename T>
 static hipError_t backward_typed(int type, const RecArgs &a, hipStream_t stream)
 {
-    const bool side = dense(type, a);
+    const bool out = dense(type, a.grad_x, a) && dense(type, a.grad_gate, a);
+    const Order x = order_of(type, a.x, a), grad = order_of(type, a.y, a);
+    const Order in = out && grad != kAny && x == order_of(type, a.gate, a) ? x : kAny;
     const Shape s = shape_of(a.batch, a.channels, a.steps, 1);
     float *partial = nullptr;
     if (a.grad_bias != nullptr)
@@ -808,8 +830,11 @@ static hipError_t backward_typed(int type, const RecArgs &a, hipStream_t stream)
     }
     const dim3 grid(s.chain ? s.tiles * s.cols : s.cols), block(s.waves * kLanes);
     kernel_log_add(s.chain ? "recurrence_backward_kernel<chain>" : "recurrence_backward_kernel", (long)grid.x * block.x);
-    if (side) FBFC_LAUNCH((recurrence_backward_kernel<T, true>), grid, block, 0, stream, a, partial);
-    else FBFC_LAUNCH((recurrence_backward_kernel<T, false>), grid, block, 0, stream, a, partial);
+    if (in == kDense && grad == kDense) FBFC_LAUNCH((recurrence_backward_kernel<T, kDense, kDense>), grid, block, 0, stream, a, partial);
+    else if (in == kDense) FBFC_LAUNCH((recurrence_backward_kernel<T, kDense, kPlanes>), grid, block, 0, stream, a, partial);
+    else if (in == kPlanes && grad == kDense) FBFC_LAUNCH((recurrence_backward_kernel<T, kPlanes, kDense>), grid, block, 0, stream, a, partial);
+    else if (in == kPlanes) FBFC_LAUNCH((recurrence_backward_kernel<T, kPlanes, kPlanes>), grid, block, 0, stream, a, partial);
+    else FBFC_LAUNCH((recurrence_backward_kernel<T, kAny, kAny>), grid, block, 0, stream, a, partial);
     const hipError_t e = hipGetLastError();
     return e != hipSuccess || partial == nullptr ? e : launch_bias(partial, (long)s.tiles * a.batch, a, stream);
 }

@@ -553,3 +553,21 @@ def test_a_captured_step_is_a_new_token_at_each_replay():
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(y, other.step([x[:, t], gate[:, t]], want)) and torch.equal(state, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("planes", ["inputs", "gradient", "all", "x"])
+@pytest.mark.parametrize("shape", [(1, 16, 64), (2, 47, 70), (3, 300, 130), (2, 1500, 33), (300, 40, 1)], ids=lambda s: "%dx%dx%d" % s)
+def test_planes_of_a_convolution_beside_rows_of_channels(shape, planes, dtype):
+    net, x, gate, gy, h0, gh = _data(*shape, TYPES[dtype], 21)
+    turn = lambda t: t.transpose(1, 2).contiguous().transpose(1, 2)   # noqa: E731
+    if planes != "gradient":
+        x = turn(x)
+    if planes in ("inputs", "all"):
+        gate = turn(gate)
+    if planes in ("gradient", "all"):
+        gy = turn(gy)
+    _check_all(net, x, gate, gy, h0, gh)
+    lengths = torch.arange(shape[0], dtype=torch.int32, device="cuda") * 17 % (shape[1] + 1)
+    _check_all(net, x, gate, gy, h0, gh, lengths)
