@@ -18,8 +18,8 @@
 // step m / sqrt(v) would have no bound.
 //
 // Measured: 40 million parameters of 160 tensors in 32 bits 222 us (5.05 TB/s, what a large copy reaches); 250 million with 16-bit
-// gradients and 8-bit states 726 us (4.84 TB/s); 25 million in bf16 with 8-bit states, unaligned, 62 us (4.06 TB/s; here
-// the arithmetic of the rounding counts, with divisions and roots rounded to half a unit 69 us).  Non-temporal stores,
+// gradients and 8-bit states 721 us (4.88 TB/s); 25 million in bf16 with 8-bit states, unaligned, 59 us (4.28 TB/s; here
+// the arithmetic counts: 62 us with the rounding in integer operations, 69 with divisions and roots rounded to half a unit too).  Non-temporal stores,
 // 1024 to 4096 workgroups and 8 or 16 parameters in flight a lane are all within 3 %; a workgroup for each piece is
 // slower with 8-bit states (783 us).  2.9 million of 126 tensors: 13.2 us with 8-bit states, 16.7 in 32 bits (30.7 and 32.7
 // where all workgroups report their end at one address).
@@ -62,7 +62,7 @@ AdamwClock adamw_clock(long t, double beta1, double beta2, unsigned seed)
 
 __global__ void adamw_set_clock_kernel(AdamwClock *clock, AdamwClock to) { *clock = to; }
 
-// Two 20-bit numbers, of the place whose product with kHash1, plus the key, is `x`.
+// Two numbers with 20 random bits on top, of the place whose product with kHash1, plus the key, is `x`.
 __device__ __forceinline__ void random_pair(unsigned x, unsigned &a, unsigned &b)
 {
     x ^= x >> 16;
@@ -73,8 +73,8 @@ __device__ __forceinline__ void random_pair(unsigned x, unsigned &a, unsigned &b
     unsigned y = x * kHash1;
     y ^= y >> 16;
     y *= kHash2;
-    a = x >> 12;
-    b = y >> 12;
+    a = x;
+    b = y;
 }
 
 // The largest magnitude of the wavefront.  The bits of magnitudes are in the order of their values, a NaN's above all.
@@ -87,13 +87,12 @@ __device__ __forceinline__ float wave_top(const float4v &v)
     return __uint_as_float(lanes_reduce<64>(top, [](unsigned a, unsigned b) { return max(a, b); }));
 }
 
-// e4m3 bits of a magnitude times `inverse`.  The bits of a 32-bit float of 2^-120 times the value hold an e4m3
-// number on top (its smallest normal number, 2^-6, becomes the float's, 2^-126), so a 20-bit random number added below
-// rounds it, subnormal numbers too.
-__device__ __forceinline__ unsigned round8(float magnitude, float inverse, unsigned random)
+// Byte I of `codes` becomes the e4m3 bits of a value of at most 448, rounded with the 20 upper bits of `random`: the
+// instruction adds them below the last bit that is kept, of subnormal numbers too.
+template <int I>
+__device__ __forceinline__ unsigned round8(float value, unsigned random, unsigned codes)
 {
-    const unsigned bits = __float_as_uint(magnitude * inverse * 0x1p-120f);
-    return min((bits + random) >> 20, 0x7Eu);
+    return __builtin_amdgcn_cvt_sr_fp8_f32(value, (int)random, (int)codes, I);
 }
 
 // scale of a block, and its inverse; a block below 2^-100 is zero
@@ -170,16 +169,17 @@ __device__ __forceinline__ void step_four(const Four<P, G, BITS> &f, const Adamw
         const float ms = scale8(wave_top(m), mi), vs = scale8(wave_top(v), vi);
         const unsigned x = (unsigned)at * kHash1 + (unsigned)((unsigned long)at >> 32) * kHash3 + key;
         unsigned mc = 0, vc = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        const auto round = [&](auto place) {
+            constexpr int I = decltype(place)::value;
             unsigned r, q;
-            random_pair(x + i * kHash1, r, q);
-            const unsigned c = round8(fabsf(m[i]), mi, r) | (m[i] < 0.0f ? 0x80u : 0u);
-            unsigned w = round8(v[i], vi, q);
-            w = v[i] > 0.0f && vi > 0.0f ? max(w, 1u) : w;
-            mc |= c << (8 * i);
-            vc |= w << (8 * i);
-        }
+            random_pair(x + I * kHash1, r, q);
+            mc = round8<I>(copysignf(fminf(fabsf(m[I]) * mi, 448.0f), m[I]), r, mc);
+            vc = round8<I>(fmaxf(fminf(v[I] * vi, 448.0f), v[I] > 0.0f && vi > 0.0f ? 0x1p-9f : 0.0f), q, vc);  // 2^-9: the smallest
+        };
+        round(std::integral_constant<int, 0>{});
+        round(std::integral_constant<int, 1>{});
+        round(std::integral_constant<int, 2>{});
+        round(std::integral_constant<int, 3>{});
         static_cast<unsigned *>(a.m)[at >> 2] = mc;
         static_cast<unsigned *>(a.v)[at >> 2] = vc;
         if ((threadIdx.x & 63) == 0) {
