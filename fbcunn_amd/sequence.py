@@ -36,7 +36,7 @@ class _Call:
     def __init__(self, like, results):
         self.shape, self.dtype, self.device, self.index = like.shape, like.dtype, like.device, like.device.index
         self.bytes = like.numel() * like.element_size()
-        self.captured = False
+        self.captured = self.capturing = False   # into any graph so far; now
         self._made = [(None, 0)] * results
 
     def result(self, i, places=()):
@@ -72,14 +72,14 @@ class _Calls:
                 self._captured.append(self._call)
             self._call, self._signature = call, now
         call = self._call
-        if torch.cuda.is_current_stream_capturing():
-            call.captured = True
+        call.capturing = torch.cuda.is_current_stream_capturing()
+        call.captured |= call.capturing
         return call
 
 
 class _RecurrenceCall(_Call):
     """Of the recurrence: checked sizes and descriptors.  Results: the output, the gradients of x and gate, the last state and the
-    gradient of the first."""
+    gradient of the first, the states that backward begins at."""
 
     def __init__(self, net, input, dims):
         x, gate = input
@@ -89,7 +89,7 @@ class _RecurrenceCall(_Call):
         if x.dim() != dims or x.size(-1) != channels:
             raise ValueError("x must be (%s%d)" % ("batch, steps, " if dims == 3 else "batch, ", channels))
         _check_device(x, net.parameters())
-        super().__init__(x, 5)
+        super().__init__(x, 6)
         self.batch, steps = x.size(0), x.size(1) if dims == 3 else 1
         desc = RecurrenceDesc(self.batch, channels, steps, TYPES[x.dtype])
         self.desc = ctypes.byref(desc)
@@ -104,6 +104,10 @@ class _RecurrenceCall(_Call):
     def state(self, i):
         t = self._made[i][0]
         return self._make(i, (self.batch, self.shape[-1]), torch.float32) if t is None else t
+
+    def checkpoints(self):
+        t = self._made[5][0]
+        return self._make(5, (self.checkpointBytes,), torch.uint8) if t is None else t
 
 
 class GatedLinearRecurrence:
@@ -127,7 +131,7 @@ class GatedLinearRecurrence:
         self.gradBias = torch.zeros(nChannels, device=self.device)
         self.train = True
         self.output = self.state = self.gradInput = self.gradState = None
-        self._workspace, self._checkpoints = Workspace(), Workspace()
+        self._workspace = Workspace()
         self._calls = {dims: _Calls(_RecurrenceCall, dims) for dims in (2, 3)}   # of step and updateOutput
         self._forward = None   # (shape, type, lengths, checkpoints) of the updateOutput that backward may follow
 
@@ -179,12 +183,13 @@ class GatedLinearRecurrence:
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
         self.output = call.result(0, places)
         self.state = call.state(3)
-        kept = self._checkpoints.take(call.checkpointBytes, call.device) if self.train else None
+        kept = call.checkpoints() if self.train else None
         call.steps[2].data = self.output.data_ptr()
         self._forward = None
         check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), first, sizes, call.refs[2],
                                             self.state.data_ptr(), kept.data_ptr() if self.train else None,
-                                            self._workspace.take(call.workspaceBytes, call.device).data_ptr(), stream))
+                                            self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr(),
+                                            stream))
         if self.train:
             self._forward = (call.shape, call.dtype, lengths, kept)
         return self.output
@@ -223,7 +228,8 @@ class GatedLinearRecurrence:
         check(lib().fbfc_recurrence_backward(call.desc, *call.refs[:2], self.bias.data_ptr(), _ptr(lengths), kept.data_ptr(),
                                              call.refs[5], last, *grads,
                                              self.gradBias.data_ptr() if weights else None, scale, first,
-                                             self._workspace.take(call.workspaceBytes, call.device).data_ptr(), stream))
+                                             self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr(),
+                                            stream))
 
     def updateGradInput(self, input, gradOutput, gradState=None):
         """[gradient of x, gradient of gate]; self.gradState is the gradient of the state before the first step.  `gradState`:
@@ -362,7 +368,7 @@ class GatedResidualNorm:
             grads[:len(input)] = [call.at(7 + i, t) for i, t in enumerate(self.gradInput)]
         ws, params = None, [None] * 3
         if weights:
-            ws = self._workspace.take(call.workspaceBytes, call.device).data_ptr()
+            ws = self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr()
             params = [None if t is None else t.data_ptr() for t in (self.gradPostWeight, self.gradScale, self.gradPreWeight)]
         check(lib().fbfc_residual_norm_backward(call.desc, *call.inputs, *self._weights(), call.at(5, gr), call.at(6, gn), *grads,
                                                 *params, scale, ws, stream))

@@ -44,16 +44,19 @@ def _check_tensor(t, name, ndim=None, strided=False):
 
 
 class Workspace:
-    """Device memory that a module hands to its calls, grown as they need more.  What was outgrown is kept: a graph
-    captured with it may still be replayed."""
+    """Device memory that a module hands to its calls, grown as they need more.  Each stream has its own, and so has each
+    call that is captured into a graph, for as long as the module lives: calls that run at the same time share none."""
 
     def __init__(self):
-        self._kept = []
+        self._of, self._captured = {}, []
 
-    def take(self, nbytes, device):
-        last = self._kept[-1] if self._kept else None
+    def take(self, nbytes, device, stream=None, capturing=False):
+        last = None if capturing else self._of.get(stream)
         if last is None or last.numel() < nbytes or last.device != device:
             size = max(nbytes, 2 * last.numel() if last is not None and last.device == device else 0, 256)
             last = torch.empty(size, dtype=torch.uint8, device=device)
-            self._kept.append(last)
+            if capturing:
+                self._captured.append(last)
+            else:
+                self._of[stream] = last
         return last

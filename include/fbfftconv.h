@@ -446,7 +446,7 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_
  * not null; that of gate_bias is the sum over sequences and steps, in a fixed order, times `factor`.  grad_state_out,
  * the gradient of state_out, may be null, or be grad_state_in.
  * `workspace`: fbfc_recurrence_workspace_bytes bytes, 16-byte aligned, of any content; calls that may run at the same
- * time need one each. */
+ * time need one each (the parts of a call wait for what other parts write there). */
 typedef struct {
     int batch, channels;
     long steps;

@@ -571,3 +571,43 @@ def test_planes_of_a_convolution_beside_rows_of_channels(shape, planes, dtype):
     _check_all(net, x, gate, gy, h0, gh)
     lengths = torch.arange(shape[0], dtype=torch.int32, device="cuda") * 17 % (shape[1] + 1)
     _check_all(net, x, gate, gy, h0, gh, lengths)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [300, 2500])
+def test_one_module_in_two_graphs_and_on_two_streams_at_once(T):
+    """The tiles of a call wait for each other through the workspace: calls that may run at the same time have one each."""
+    net, x, gate, gy, h0, gh = _data(2, T, 70, torch.float32, 22)
+
+    def step():
+        net.updateOutput([x, gate], state=h0)
+        net.backward([x, gate], gy, gradState=gh)
+
+    step()
+    results = [net.output, net.state, *net.gradInput, net.gradState, net.gradBias]
+    want = [t.clone() for t in results]
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    for g in graphs:
+        with torch.cuda.graph(g):
+            step()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        with torch.cuda.stream(s):
+            step()
+    torch.cuda.synchronize()
+    used = [w.data_ptr() for w in net._workspace._captured] + [w.data_ptr() for w in net._workspace._of.values()]
+    assert len(used) == len(set(used)) == 2 * 2 + 3
+    for rep in range(3):
+        for t in results:
+            t.fill_(float("nan"))
+        torch.cuda.synchronize()
+        for s, g in zip(streams, graphs):   # the same inputs and results, so they agree whatever runs first
+            with torch.cuda.stream(s):
+                g.replay()
+        step()
+        for s in streams:
+            with torch.cuda.stream(s):
+                step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(results, want)), rep
