@@ -319,6 +319,12 @@ __device__ __forceinline__ long length_of(const int *lengths, int b, long steps)
     return n < 0 ? 0 : n < steps ? n : steps;
 }
 
+// Backward keeps a gate as 1 - a, or as -a where a is the smaller, so that the smaller of the two has its full precision.  The
+// sign bit tells them apart, not the value: for a gate below -87 e^z underflows, and -a is -0.
+__device__ __forceinline__ bool holds_a(float m) { return __float_as_int(m) < 0; }
+__device__ __forceinline__ float closed_of(float m) { return holds_a(m) ? 1.0f + m : m; }
+__device__ __forceinline__ float open_of(float m) { return holds_a(m) ? -m : 1.0f - m; }
+
 // How many of the 16 steps from t0 on lie before `end`.
 __device__ __forceinline__ int steps_before(long t0, long end) { return (int)(end - t0 < 0 ? 0 : end - t0 < kRun ? end - t0 : kRun); }
 
@@ -532,7 +538,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
         const int n = steps_before(t0, len), n_all = steps_before(t0, steps);
         const bool full = n == kRun && whole;
         Vec<T, V> x[kRun], gy[kRun];
-        float m[kRun][V], before[V];  // m: 1 - a, or -a where that is less: the smaller of the two has its full precision
+        float m[kRun][V], before[V];  // m: see holds_a()
         float A[V], S[V], R[V];       // product of the a, state behind these steps, a u of the first of them, from zero
 #pragma unroll
         for (int i = 0; i < V; ++i)
@@ -613,9 +619,8 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
             forget<T, V>(x[t]);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float k = m[t][i] < 0.0f ? 1.0f + m[t][i] : m[t][i];
                 d[t][i] = before[i] - (float)x[t][i];
-                before[i] = fmaf(-k, d[t][i], before[i]);
+                before[i] = fmaf(-closed_of(m[t][i]), d[t][i], before[i]);
             }
             if (t % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
@@ -649,8 +654,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_backward_kernel(
                 float gx[V], gz[V];
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    const bool small = m[t][i] < 0.0f;
-                    const float k = small ? 1.0f + m[t][i] : m[t][i], keep = small ? -m[t][i] : 1.0f - m[t][i];
+                    const float k = closed_of(m[t][i]), keep = open_of(m[t][i]);
                     const float u = (float)gy[t][i] + g[i];
                     gx[i] = k * u;
                     g[i] = keep * u;

@@ -611,3 +611,69 @@ def test_one_module_in_two_graphs_and_on_two_streams_at_once(T):
                 step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(results, want)), rep
+
+
+def _closed(dtype):
+    """Gates that replace the state, or keep it: around where e^z leaves the normal numbers, and far beyond."""
+    return [-80.0, -86.0, -87.0, -88.0, -104.0, -300.0, torch.finfo(dtype).min, -float("inf"), 88.0, 300.0, float("inf")]
+
+
+def _close(gate, T):
+    """Channel (i, j) of `gate` has value i of _closed() at place j: the ends of a run of 16 steps, of a tile of 128, of the
+    sequence, their neighbours, and a whole run.  {place: steps}"""
+    places = [[t] for t in (0, 1, 15, 16, 40, 127, 128, T - 1) if t < T] + [list(range(32, 48))] * (T >= 48)
+    values = _closed(gate.dtype)
+    for j, steps in enumerate(places):
+        for i, v in enumerate(values):
+            gate[:, steps, j * len(values) + i] = v
+    return places
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("padded", [False, True])
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("shape,order", [((2, 1, 25), "btd"), ((3, 16, 45), "btd"), ((2, 300, 101), "btd"), ((3, 700, 101), "bdt"),
+                                         ((2, 300, 101), "tbd"), ((130, 300, 101), "btd")], ids=str)
+def test_gradients_at_closed_gates(shape, order, dtype, padded):
+    """The bounds of _plain() hold for gates below 10.  At the others here the smaller of a and 1 - a is below 2e-35.  Its relative
+    error is below 2^-15: |z| + 2 units of 2^-24 for up to 104, and zero in its place below 2^-126.  So it is off by less than 2^-126,
+    and a result, which is a sum of at most B T products of it with one u and one d, by less than 2^-126 B T |u| |d|, where
+    |u| <= |gh| + T max |gy|, and |d| <= 2 max(|x|, |h0|) because a state lies between those."""
+    net, x, gate, gy, h0, gh = _data(*shape, TYPES[dtype], 23, order)
+    net.bias.zero_()
+    _close(gate, shape[1])
+    lengths = None
+    if padded:   # the full length, one step less, which ends before the gate of the last one, and so on
+        lengths = (shape[1] - torch.arange(shape[0], device="cuda") % 3 * (shape[1] // 3)).to(torch.int32)
+        lengths[1] = shape[1] - 1
+    want = _plain(x, gate, net.bias, h0, lengths, gy, gh)
+    top = lambda *t: max(1.0, *(float(v.abs().max()) for v in t))   # noqa: E731
+    under = 2.0 ** -126 * shape[0] * shape[1] * (shape[1] + 1) * top(gy, gh) * 2 * top(x, h0)
+    assert under < 1e-28   # nothing beside the other roundings
+    y = net.updateOutput([x, gate], state=h0, lengths=lengths)
+    net.backward([x, gate], gy, gradState=gh)
+    for name, got in (("output", y), ("state", net.state), ("gradX", net.gradInput[0]), ("gradGate", net.gradInput[1]),
+                      ("gradState", net.gradState), ("gradBias", net.gradBias)):
+        _check(got, (want[name][0], want[name][1] + under), name)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape", [(2, 300, 101), (130, 300, 101)], ids=str)
+def test_no_gradient_passes_a_closed_gate(shape):
+    net, x, gate, gy, h0, gh = _data(*shape, torch.float32, 24)
+    net.bias.zero_()
+    values, places = _closed(torch.float32), _close(gate, shape[1])
+    net.updateOutput([x, gate], state=h0)
+    first = [t.clone() for t in net.backward([x, gate], gy, gradState=gh)] + [net.gradState.clone()]
+    after = torch.zeros(shape, dtype=torch.bool, device="cuda")
+    for j, steps in enumerate(places):
+        for i, v in enumerate(values):
+            if v <= -104:
+                after[:, steps[-1]:, j * len(values) + i] = True
+    other = torch.where(after, gy * 2 + 1, gy)
+    again = net.backward([x, gate], other, gradState=torch.where(after[:, -1], gh * 2 + 1, gh)) + [net.gradState]
+    for a, b in zip(first[:2], again[:2]):   # of the steps before the gate
+        assert torch.equal(torch.where(after, 0, a), torch.where(after, 0, b))
+    closed = after.any(1)
+    assert torch.equal(first[2][closed], again[2][closed])
+    assert not torch.equal(first[0], again[0])
