@@ -38,6 +38,7 @@ class _Call:
         self.bytes = like.numel() * like.element_size()
         self.captured = self.capturing = False   # into any graph so far; now
         self._made = [(None, 0)] * results
+        self._written, self._kept = [False] * results, []   # which of them a graph writes to; those that were replaced
 
     def result(self, i, places=()):
         """Result i, the tensor of the last call unless one of `places` lies in it: an input that is a module's last
@@ -48,12 +49,16 @@ class _Call:
                 if at <= p < at + self.bytes:
                     break
             else:
+                self._written[i] |= self.capturing
                 return t
         return self._make(i, self.shape, self.dtype)
 
     def _make(self, i, shape, dtype):
+        if self._written[i]:
+            self._kept.append(self._made[i][0])
         t = torch.empty(shape, dtype=dtype, device=self.device)
         self._made[i] = t, t.data_ptr()
+        self._written[i] = self.capturing
         return t
 
 

@@ -677,3 +677,47 @@ def test_no_gradient_passes_a_closed_gate(shape):
     closed = after.any(1)
     assert torch.equal(first[2][closed], again[2][closed])
     assert not torch.equal(first[0], again[0])
+
+
+def test_a_result_that_a_graph_writes_to_is_kept_when_another_takes_its_place():
+    import weakref
+    from fbcunn_amd.sequence import _Call
+    call = _Call(torch.zeros(4, 5), 1)
+    alive = lambda refs: [r() is not None for r in refs]   # noqa: E731
+    first = call.result(0)
+    call.captured = call.capturing = True
+    assert call.result(0) is first                       # made before the capture, written in it
+    second = call.result(0, [first.data_ptr()])          # an input of the captured call itself
+    call.capturing = False
+    third = call.result(0, [second.data_ptr()])          # an input of a later call
+    fourth = call.result(0, [third.data_ptr() + 4])      # no graph writes to the third
+    refs = [weakref.ref(t) for t in (first, second, third, fourth)]
+    del first, second, third, fourth
+    assert alive(refs) == [True, True, False, True]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("twice", [True, False])
+def test_a_graph_keeps_results_that_were_its_modules_inputs(twice):
+    """A module applied twice in a captured step, or eagerly to what a captured step gave; all references dropped, memory
+    that was given back would be found by the fill."""
+    net, x, gate, *_ = _data(2, 150, 40, torch.float32, 25)
+    other, *_ = _data(2, 150, 40, torch.float32, 25)
+    apply = lambda m: m.updateOutput([m.updateOutput([x, gate]) if twice else x, gate])   # noqa: E731
+    apply(net)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = apply(net)
+    if not twice:
+        net.updateOutput([net.updateOutput([y, gate]), gate])
+    seen = y.data_ptr()
+    del y
+    fill = [torch.full((2 * 150 * 40,), 7.0, device="cuda") for _ in range(40)]
+    assert seen not in [t.data_ptr() for t in fill]
+    for rep in range(3):
+        x.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(bool((t == 7.0).all()) for t in fill), rep
+        apply(other)
