@@ -41,21 +41,22 @@ class _Call:
         self._written, self._kept = [False] * results, []   # which of them a graph writes to; those that were replaced
 
     def result(self, i, places=()):
-        """Result i, the tensor of the last call unless one of `places` lies in it: an input that is a module's last
-        output, or a view of it, keeps its values, which backward reads."""
+        """Result i, of the inputs' shape and type.  `places`: the addresses of what the call reads."""
+        return self._result(i, self.shape, self.dtype, self.bytes, places)
+
+    def _result(self, i, shape, dtype, nbytes, places):
+        """The tensor of the last call unless one of `places` lies in it: an input that is a module's last result, or a
+        view of it, keeps its values, which backward, or its other half, reads."""
         t, at = self._made[i]
         if t is not None:
             for p in places:
-                if at <= p < at + self.bytes:
+                if at <= p < at + nbytes:
                     break
             else:
                 self._written[i] |= self.capturing
                 return t
-        return self._make(i, self.shape, self.dtype)
-
-    def _make(self, i, shape, dtype):
         if self._written[i]:
-            self._kept.append(self._made[i][0])
+            self._kept.append(t)
         t = torch.empty(shape, dtype=dtype, device=self.device)
         self._made[i] = t, t.data_ptr()
         self._written[i] = self.capturing
@@ -106,13 +107,11 @@ class _RecurrenceCall(_Call):
         self.steps = [Steps(0, *s) for s in (strides[0], strides[1], whole, whole, whole, whole)]
         self.refs = [ctypes.byref(s) for s in self.steps]
 
-    def state(self, i):
-        t = self._made[i][0]
-        return self._make(i, (self.batch, self.shape[-1]), torch.float32) if t is None else t
+    def state(self, i, places):
+        return self._result(i, (self.batch, self.shape[-1]), torch.float32, self.batch * self.shape[-1] * 4, places)
 
     def checkpoints(self):
-        t = self._made[5][0]
-        return self._make(5, (self.checkpointBytes,), torch.uint8) if t is None else t
+        return self._result(5, (self.checkpointBytes,), torch.uint8, self.checkpointBytes, ())
 
 
 class GatedLinearRecurrence:
@@ -125,7 +124,7 @@ class GatedLinearRecurrence:
     updateGradInput and accGradParameters) follows an updateOutput of the same inputs, from which the module keeps the
     state before every 128 steps; after evaluate() it keeps none and cannot go backward.  step advances sequences by one
     token.  As in the other modules the outputs are the module's own tensors, which its next call on inputs of the same
-    shape writes again, unless they are its inputs."""
+    shape writes again, unless they are its inputs; a `state` that is its self.state is advanced in place."""
 
     def __init__(self, nChannels, device="cuda"):
         if not isinstance(nChannels, int) or nChannels < 1:
@@ -187,7 +186,7 @@ class GatedLinearRecurrence:
         call, places, stream = self._call(input, 3)
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
         self.output = call.result(0, places)
-        self.state = call.state(3)
+        self.state = call.state(3, places)
         kept = call.checkpoints() if self.train else None
         call.steps[2].data = self.output.data_ptr()
         self._forward = None
@@ -214,21 +213,22 @@ class GatedLinearRecurrence:
         return self.output
 
     def _backward(self, input, gradOutput, gradState, inputs, weights, scale):
-        call, _, stream = self._call(input, 3)
+        call, places, stream = self._call(input, 3)
         shape, dtype, lengths, kept = self._forward or (None, None, None, None)
         if shape != call.shape or dtype != call.dtype or kept.device != call.device:
             raise ValueError("backward follows an updateOutput of the same inputs, not after evaluate()")
         _check_activation(gradOutput, "gradOutput", call)
         last = self._check_state(gradState, "gradState", call)
         of = call.steps[5]
-        of.data = gradOutput.data_ptr()
+        of.data = at = gradOutput.data_ptr()
         of.stride_batch, of.stride_step, of.stride_channel = gradOutput.stride()
         grads, first = (None, None), None
         if inputs:
-            self.gradInput = [call.result(1), call.result(2)]
+            places += (at, last or 0)
+            self.gradInput = [call.result(1, places), call.result(2, places)]
             call.steps[3].data, call.steps[4].data = (t.data_ptr() for t in self.gradInput)
             grads = call.refs[3:5]
-            self.gradState = call.state(4)
+            self.gradState = call.state(4, places)
             first = self.gradState.data_ptr()
         check(lib().fbfc_recurrence_backward(call.desc, *call.refs[:2], self.bias.data_ptr(), _ptr(lengths), kept.data_ptr(),
                                              call.refs[5], last, *grads,
@@ -357,7 +357,7 @@ class GatedResidualNorm:
         return [None if t is None else t.data_ptr() for t in (self.postWeight, self.scale, self.preWeight)]
 
     def _backward(self, input, gradOutput, inputs, weights, scale):
-        call, input, _, stream = self._call(input)
+        call, input, places, stream = self._call(input)
         gr, gn = gradOutput
         if gr is None and gn is None:
             raise ValueError("gradOutput is [gradOutput, gradNormed], and one of them is needed")
@@ -367,9 +367,10 @@ class GatedResidualNorm:
             if t is not None:
                 _check_activation(t, name, call)
                 call.rows[i].stride = self._row_stride(t, name)
+                places.append(t.data_ptr())
         grads = [None] * 3
         if inputs:
-            self.gradInput = [call.result(2 + i) for i in range(len(input))]
+            self.gradInput = [call.result(2 + i, places) for i in range(len(input))]
             grads[:len(input)] = [call.at(7 + i, t) for i, t in enumerate(self.gradInput)]
         ws, params = None, [None] * 3
         if weights:

@@ -721,3 +721,52 @@ def test_a_graph_keeps_results_that_were_its_modules_inputs(twice):
         torch.cuda.synchronize()
         assert all(bool((t == 7.0).all()) for t in fill), rep
         apply(other)
+
+
+def _same(net, other, what):
+    results = lambda m: [m.output, m.state, *m.gradInput, m.gradState, m.gradBias]   # noqa: E731
+    for i, (a, b) in enumerate(zip(results(net), results(other))):
+        assert torch.equal(a, b), (what, i)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [40, 700])
+def test_own_gradients_and_states_as_inputs_keep_their_values(T):
+    """What the module's last call gave is an input of the next, whose halves both have to find it as it was."""
+    net, x, gate, gy, h0, gh = _data(2, T, 40, torch.float32, 26)
+    other, *_ = _data(2, T, 40, torch.float32, 26)
+
+    def halves(m, inputs, grad):
+        m.updateOutput(inputs, state=h0)
+        m.updateGradInput(inputs, grad, gh)
+        m.accGradParameters(inputs, grad, 1.0, gh)
+
+    halves(net, [x, gate], gy)
+    for i in range(2):
+        mine = net.gradInput[i]
+        kept = mine.clone()
+        halves(net, [x, gate], mine)         # a gradient of the output
+        halves(other, [x, gate], kept)
+        assert torch.equal(mine, kept)
+        _same(net, other, ("gradOutput", i))
+        mine = net.gradInput[i]
+        kept = mine.clone()
+        halves(net, [mine, gate], gy)        # an input
+        halves(other, [kept, gate], gy)
+        assert torch.equal(mine, kept)
+        _same(net, other, ("input", i))
+    mine = net.gradState
+    kept = mine.clone()
+    net.updateGradInput([x, gate], gy, mine), net.accGradParameters([x, gate], gy, 1.0, mine)
+    other.updateGradInput([x, gate], gy, kept), other.accGradParameters([x, gate], gy, 1.0, kept)
+    assert torch.equal(mine, kept)
+    _same(net, other, "gradState")
+    last = lambda m: m.updateOutput([x[:, :1], gate[:, :1]], state=h0)   # noqa: E731
+    last(net), last(other)
+    for name in ("state", "state", "gradState"):           # a state as a sequence of one step
+        mine = getattr(net, name)
+        kept = mine.clone()
+        halves(net, [mine[:, None], gate[:, :1]], gy[:, :1])
+        halves(other, [kept[:, None], gate[:, :1]], gy[:, :1])
+        assert torch.equal(mine, kept)
+        _same(net, other, name)

@@ -469,3 +469,27 @@ def test_a_graph_keeps_its_results_when_the_module_goes_on_with_other_shapes():
         step(other)
         assert torch.equal(out, other.output[0]) and torch.equal(normed, other.output[1])
         assert torch.equal(net.gradScale, other.gradScale)
+
+
+@pytest.mark.gpu
+def test_own_gradients_as_inputs_keep_their_values():
+    """What the module's last call gave is an input of the next, whose halves both have to find it as it was."""
+    net, other = _net(48, "full", 1), _net(48, "full", 1)
+    inputs, grads = _inputs((6, 48), "full", torch.float32, 8)
+
+    def halves(m, inputs, grads):
+        m.updateOutput(inputs)
+        m.updateGradInput(inputs, grads)
+        m.accGradParameters(inputs, grads)
+
+    halves(net, inputs, grads)
+    for i in range(3):
+        for place in range(5):
+            mine = net.gradInput[i]
+            kept = mine.clone()
+            given = [(inputs + grads)[:place] + [t] + (inputs + grads)[place + 1:] for t in (mine, kept)]
+            halves(net, given[0][:3], given[0][3:])
+            halves(other, given[1][:3], given[1][3:])
+            assert torch.equal(mine, kept), (i, place)
+            for a, b in zip(net.output + net.gradInput + net.parameters()[1], other.output + other.gradInput + other.parameters()[1]):
+                assert torch.equal(a, b), (i, place)
