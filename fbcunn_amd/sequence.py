@@ -6,7 +6,7 @@ import torch
 
 from . import _lib
 from ._lib import RecurrenceDesc, ResidualNormDesc, Rows, Steps, check, lib
-from .tensors import TYPES, Workspace, _ptr, signature, stream_on
+from .tensors import TYPES, Workspace, _ptr, is_capturing, signature, stream_on
 
 __all__ = ["GatedLinearRecurrence", "GatedResidualNorm"]
 
@@ -25,9 +25,21 @@ def _check_activation(t, name, like=None):
             raise ValueError("%s is on another device" % name)
 
 
-def _check_device(t, parameters):
-    if any(p.device != t.device for tensors in parameters for p in tensors):
-        raise ValueError("the inputs are on another device than the parameters")
+def _parameter(t, name, channels, index):
+    """The address of a parameter or its gradient; None for an absent one.  Looked at in each call, since any tensor may have
+    been assigned to it."""
+    if t is None:
+        return None
+    try:
+        if t.dtype is torch.float32 and t.numel() == channels and t.is_contiguous() and t.get_device() == index:
+            return t.data_ptr()
+    except AttributeError:
+        raise TypeError("%s must be a tensor" % name) from None
+    if t.dtype is not torch.float32:
+        raise TypeError("%s must be float32" % name)
+    if t.get_device() != index:
+        raise ValueError("%s is on another device than the inputs" % name)
+    raise ValueError("%s must be %d contiguous numbers" % (name, channels))
 
 
 class _Call:
@@ -35,32 +47,35 @@ class _Call:
 
     def __init__(self, like, results):
         self.shape, self.dtype, self.device, self.index = like.shape, like.dtype, like.device, like.device.index
-        self.bytes = like.numel() * like.element_size()
         self.captured = self.capturing = False   # into any graph so far; now
-        self._made = [(None, 0)] * results
+        self._made = [(None, 0, 0)] * results
         self._written, self._kept = [False] * results, []   # which of them a graph writes to; those that were replaced
 
     def result(self, i, places=()):
-        """Result i, of the inputs' shape and type.  `places`: the addresses of what the call reads."""
-        return self._result(i, self.shape, self.dtype, self.bytes, places)
+        """Result i, the tensor of the last call unless one of `places`, the addresses of what this call reads, lies in it: an
+        input that is a module's last result, or a view of it, keeps its values, which backward, or its other half, reads."""
+        t, at, end = self._made[i]
+        if t is None:
+            return self._make(i)
+        for p in places:
+            if at <= p < end:
+                return self._make(i)
+        if self.capturing:
+            self._written[i] = True
+        return t
 
-    def _result(self, i, shape, dtype, nbytes, places):
-        """The tensor of the last call unless one of `places` lies in it: an input that is a module's last result, or a
-        view of it, keeps its values, which backward, or its other half, reads."""
-        t, at = self._made[i]
-        if t is not None:
-            for p in places:
-                if at <= p < at + nbytes:
-                    break
-            else:
-                self._written[i] |= self.capturing
-                return t
+    def _make(self, i):
         if self._written[i]:
-            self._kept.append(t)
+            self._kept.append(self._made[i][0])
+        shape, dtype = self._like(i)
         t = torch.empty(shape, dtype=dtype, device=self.device)
-        self._made[i] = t, t.data_ptr()
+        at = t.data_ptr()
+        self._made[i] = t, at, at + t.numel() * t.element_size()
         self._written[i] = self.capturing
         return t
+
+    def _like(self, i):
+        return self.shape, self.dtype
 
 
 class _Calls:
@@ -78,7 +93,7 @@ class _Calls:
                 self._captured.append(self._call)
             self._call, self._signature = call, now
         call = self._call
-        call.capturing = torch.cuda.is_current_stream_capturing()
+        call.capturing = is_capturing()
         call.captured |= call.capturing
         return call
 
@@ -94,7 +109,6 @@ class _RecurrenceCall(_Call):
         _check_activation(gate, "gate", x)
         if x.dim() != dims or x.size(-1) != channels:
             raise ValueError("x must be (%s%d)" % ("batch, steps, " if dims == 3 else "batch, ", channels))
-        _check_device(x, net.parameters())
         super().__init__(x, 6)
         self.batch, steps = x.size(0), x.size(1) if dims == 3 else 1
         desc = RecurrenceDesc(self.batch, channels, steps, TYPES[x.dtype])
@@ -107,11 +121,10 @@ class _RecurrenceCall(_Call):
         self.steps = [Steps(0, *s) for s in (strides[0], strides[1], whole, whole, whole, whole)]
         self.refs = [ctypes.byref(s) for s in self.steps]
 
-    def state(self, i, places):
-        return self._result(i, (self.batch, self.shape[-1]), torch.float32, self.batch * self.shape[-1] * 4, places)
-
-    def checkpoints(self):
-        return self._result(5, (self.checkpointBytes,), torch.uint8, self.checkpointBytes, ())
+    def _like(self, i):
+        if i < 3:
+            return self.shape, self.dtype
+        return ((self.batch, self.shape[-1]), torch.float32) if i < 5 else ((self.checkpointBytes,), torch.uint8)
 
 
 class GatedLinearRecurrence:
@@ -184,13 +197,14 @@ class GatedLinearRecurrence:
 
     def updateOutput(self, input, state=None, lengths=None):
         call, places, stream = self._call(input, 3)
+        bias = _parameter(self.bias, "bias", self.nChannels, call.index)
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
         self.output = call.result(0, places)
-        self.state = call.state(3, places)
-        kept = call.checkpoints() if self.train else None
+        self.state = call.result(3, places)
+        kept = call.result(5) if self.train else None
         call.steps[2].data = self.output.data_ptr()
         self._forward = None
-        check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), first, sizes, call.refs[2],
+        check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], bias, first, sizes, call.refs[2],
                                             self.state.data_ptr(), kept.data_ptr() if self.train else None,
                                             self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr(),
                                             stream))
@@ -205,10 +219,10 @@ class GatedLinearRecurrence:
         call, places, stream = self._call(input, 2)
         if state is None:
             raise TypeError("step needs the state that it advances")
-        at = self._check_state(state, "state", call)
+        bias, at = _parameter(self.bias, "bias", self.nChannels, call.index), self._check_state(state, "state", call)
         self.output = call.result(0, places)
         call.steps[2].data = self.output.data_ptr()
-        check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], self.bias.data_ptr(), at, None, call.refs[2], at, None,
+        check(lib().fbfc_recurrence_forward(call.desc, *call.refs[:2], bias, at, None, call.refs[2], at, None,
                                             None, stream))
         return self.output
 
@@ -219,6 +233,8 @@ class GatedLinearRecurrence:
             raise ValueError("backward follows an updateOutput of the same inputs, not after evaluate()")
         _check_activation(gradOutput, "gradOutput", call)
         last = self._check_state(gradState, "gradState", call)
+        bias = _parameter(self.bias, "bias", self.nChannels, call.index)
+        gradBias = _parameter(self.gradBias, "gradBias", self.nChannels, call.index) if weights else None
         of = call.steps[5]
         of.data = at = gradOutput.data_ptr()
         of.stride_batch, of.stride_step, of.stride_channel = gradOutput.stride()
@@ -228,11 +244,10 @@ class GatedLinearRecurrence:
             self.gradInput = [call.result(1, places), call.result(2, places)]
             call.steps[3].data, call.steps[4].data = (t.data_ptr() for t in self.gradInput)
             grads = call.refs[3:5]
-            self.gradState = call.state(4, places)
+            self.gradState = call.result(4, places)
             first = self.gradState.data_ptr()
-        check(lib().fbfc_recurrence_backward(call.desc, *call.refs[:2], self.bias.data_ptr(), _ptr(lengths), kept.data_ptr(),
-                                             call.refs[5], last, *grads,
-                                             self.gradBias.data_ptr() if weights else None, scale, first,
+        check(lib().fbfc_recurrence_backward(call.desc, *call.refs[:2], bias, _ptr(lengths), kept.data_ptr(),
+                                             call.refs[5], last, *grads, gradBias, scale, first,
                                              self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr(),
                                             stream))
 
@@ -261,7 +276,6 @@ class _NormCall(_Call):
             raise ValueError("residual must have %d channels last" % net.nChannels)
         for t, name in zip(input[1:], net._names[1:]):
             _check_activation(t, name, residual)
-        _check_device(residual, net.parameters())
         super().__init__(residual, 2 + len(input))
         self.sizes = ResidualNormDesc(residual.numel() // net.nChannels, net.nChannels, TYPES[residual.dtype], net.eps)
         self.desc = ctypes.byref(self.sizes)
@@ -337,24 +351,33 @@ class GatedResidualNorm:
             raise ValueError("the input is [%s]" % ", ".join(self._names))
         call = self._calls.of(self, input)
         call.sizes.eps = self.eps
-        places = [t.data_ptr() for t in input]
-        for rows, p in zip(call.rows, places):
-            rows.data = p
+        places = []
+        for rows, t in zip(call.rows, input):
+            rows.data = p = t.data_ptr()
+            places.append(p)
         return call, input, places, stream_on(call.index)
 
     def updateOutput(self, input):
         call, input, places, stream = self._call(input)
+        weights = self._weights(call)
         output = call.result(0, places) if self.hasBranch else None
         normed = call.result(1, places) if self.hasNorm else None
-        check(lib().fbfc_residual_norm_forward(call.desc, *call.inputs, *self._weights(), call.at(3, output), call.at(4, normed),
+        check(lib().fbfc_residual_norm_forward(call.desc, *call.inputs, *weights, call.at(3, output), call.at(4, normed),
                                                stream))
         self.output = [output if self.hasBranch else input[0], normed]
         return self.output
 
     forward = updateOutput
 
-    def _weights(self):
-        return [None if t is None else t.data_ptr() for t in (self.postWeight, self.scale, self.preWeight)]
+    def _weights(self, call):
+        n, index = self.nChannels, call.index
+        return (_parameter(self.postWeight, "postWeight", n, index), _parameter(self.scale, "scale", n, index),
+                _parameter(self.preWeight, "preWeight", n, index))
+
+    def _gradWeights(self, call):
+        n, index = self.nChannels, call.index
+        return (_parameter(self.gradPostWeight, "gradPostWeight", n, index), _parameter(self.gradScale, "gradScale", n, index),
+                _parameter(self.gradPreWeight, "gradPreWeight", n, index))
 
     def _backward(self, input, gradOutput, inputs, weights, scale):
         call, input, places, stream = self._call(input)
@@ -368,15 +391,13 @@ class GatedResidualNorm:
                 _check_activation(t, name, call)
                 call.rows[i].stride = self._row_stride(t, name)
                 places.append(t.data_ptr())
+        values, params = self._weights(call), self._gradWeights(call) if weights else [None] * 3
         grads = [None] * 3
         if inputs:
             self.gradInput = [call.result(2 + i, places) for i in range(len(input))]
             grads[:len(input)] = [call.at(7 + i, t) for i, t in enumerate(self.gradInput)]
-        ws, params = None, [None] * 3
-        if weights:
-            ws = self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr()
-            params = [None if t is None else t.data_ptr() for t in (self.gradPostWeight, self.gradScale, self.gradPreWeight)]
-        check(lib().fbfc_residual_norm_backward(call.desc, *call.inputs, *self._weights(), call.at(5, gr), call.at(6, gn), *grads,
+        ws = self._workspace.take(call.workspaceBytes, call.device, stream, call.capturing).data_ptr() if weights else None
+        check(lib().fbfc_residual_norm_backward(call.desc, *call.inputs, *values, call.at(5, gr), call.at(6, gn), *grads,
                                                 *params, scale, ws, stream))
 
     def updateGradInput(self, input, gradOutput):

@@ -5,6 +5,8 @@ import torch
 
 from . import _lib
 
+is_capturing = torch._C._cuda_isCurrentStreamCapturing   # what torch.cuda.is_current_stream_capturing() returns
+
 TYPES = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -20,16 +22,16 @@ def _stream():
 def signature(*tensors):
     """What a call's argument checks and descriptors depend on: equal signatures need neither again."""
     try:
-        return [(t.shape, t.stride(), t.dtype, t.device) for t in tensors]
+        return [(t.shape, t.stride(), t.dtype, t.get_device()) for t in tensors]
     except AttributeError:
         raise TypeError("CUDA tensors are needed") from None
 
 
-def stream_on(index):
+def stream_on(index, device=torch._C._cuda_getDevice, stream=torch._C._cuda_getCurrentRawStream):
     """The current stream, if device `index` is the current one."""
-    if torch._C._cuda_getDevice() != index:
+    if device() != index:
         raise ValueError("the tensors are not on the current device")
-    return torch._C._cuda_getCurrentRawStream(index)
+    return stream(index)
 
 
 def _check_tensor(t, name, ndim=None, strided=False):

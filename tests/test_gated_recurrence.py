@@ -770,3 +770,39 @@ def test_own_gradients_and_states_as_inputs_keep_their_values(T):
         halves(other, [kept[:, None], gate[:, :1]], gy[:, :1])
         assert torch.equal(mine, kept)
         _same(net, other, name)
+
+
+def test_parameters_are_looked_at_in_each_call():
+    """An address goes on only of as many 32-bit numbers, side by side, on the inputs' device."""
+    from fbcunn_amd.sequence import _parameter
+    t = torch.zeros(8)
+    assert _parameter(t, "bias", 8, -1) == t.data_ptr() and _parameter(None, "bias", 8, -1) is None
+    for bad, index, error, text in ((t[:7], -1, ValueError, "8 contiguous"), (torch.zeros(9), -1, ValueError, "8 contiguous"),
+                                    (torch.zeros(16)[::2], -1, ValueError, "8 contiguous"), (t.half(), -1, TypeError, "float32"),
+                                    (t.double(), -1, TypeError, "float32"), (t, 0, ValueError, "another device"), ([0.0] * 8, -1, TypeError, "tensor")):
+        with pytest.raises(error, match=text):
+            _parameter(bad, "bias", 8, index)
+
+
+@pytest.mark.gpu
+def test_parameters_that_do_not_fit_are_refused():
+    net, x, gate, gy, h0, _ = _data(2, 5, 8, torch.float32, 27)
+    net.updateOutput([x, gate])
+    net.backward([x, gate], gy)
+    net.step([x[:, 0], gate[:, 0]], h0)
+    whole = net.bias, net.gradBias
+    for bad, error in ((whole[0].half(), TypeError), (whole[0][:7], ValueError), (whole[0].cpu(), ValueError)):
+        net.bias = bad
+        for call in (lambda: net.updateOutput([x, gate]), lambda: net.backward([x, gate], gy), lambda: net.step([x[:, 0], gate[:, 0]], h0)):
+            with pytest.raises(error, match="bias"):
+                call()
+        net.bias, net.gradBias = whole[0], bad
+        net.updateOutput([x, gate])
+        net.updateGradInput([x, gate], gy)
+        for call in (lambda: net.backward([x, gate], gy), lambda: net.accGradParameters([x, gate], gy)):
+            with pytest.raises(error, match="gradBias"):
+                call()
+        net.gradBias = whole[1]
+    net.bias.data = net.bias.data.half()       # the same tensor, of another type
+    with pytest.raises(TypeError, match="bias"):
+        net.updateOutput([x, gate])

@@ -493,3 +493,25 @@ def test_own_gradients_as_inputs_keep_their_values():
             assert torch.equal(mine, kept), (i, place)
             for a, b in zip(net.output + net.gradInput + net.parameters()[1], other.output + other.gradInput + other.parameters()[1]):
                 assert torch.equal(a, b), (i, place)
+
+
+@pytest.mark.gpu
+def test_parameters_that_do_not_fit_are_refused():
+    net = _net(48, "full", 1)
+    inputs, grads = _inputs((6, 48), "full", torch.float32, 9)
+    net.updateOutput(inputs)
+    net.backward(inputs, grads)
+    for name in ("postWeight", "scale", "preWeight", "gradPostWeight", "gradScale", "gradPreWeight"):
+        whole = getattr(net, name)
+        for bad, error in ((whole.half(), TypeError), (whole[:47], ValueError), (whole.cpu(), ValueError), (list(whole), TypeError)):
+            setattr(net, name, bad)
+            with pytest.raises(error, match=name):
+                net.backward(inputs, grads)
+            with pytest.raises(error, match=name):
+                net.accGradParameters(inputs, grads)
+            if not name.startswith("grad"):
+                with pytest.raises(error, match=name):
+                    net.updateOutput(inputs)
+        setattr(net, name, whole)
+    net.updateOutput(inputs)
+    net.backward(inputs, grads)
