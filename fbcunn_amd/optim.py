@@ -94,13 +94,15 @@ class AdamW:
         for x, y, name in zip(given, mine, ("m", "v", "mScale", "vScale")):
             if (x is None) != (y is None):
                 raise ValueError("%s does not go with %d-bit states" % (name, self.stateBits))
+            if x is not None and not isinstance(x, torch.Tensor):
+                raise TypeError("%s must be a tensor" % name)
             if x is not None and (x.dtype != y.dtype or x.shape != y.shape):
                 raise ValueError("%s must be %s of shape %s" % (name, y.dtype, tuple(y.shape)))
+        with torch.cuda.device(self.device):
+            check(lib().fbfc_adamw_set_step(self._handle, t, _stream()))   # refuses a number of steps before anything is copied
         for x, y in zip(given, mine):
             if x is not None:
                 y.copy_(x)
-        with torch.cuda.device(self.device):
-            check(lib().fbfc_adamw_set_step(self._handle, t, _stream()))
 
     def close(self):
         if self._handle:

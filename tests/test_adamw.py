@@ -373,3 +373,18 @@ def test_more_than_32_bits_of_parameters():
     assert bool(((value - want).abs() <= 2.0 ** -3 * want.abs() + opt.mScale[cut // 256:, None] * 2.0 ** -9).all())   # one spacing
     assert not torch.equal(p[cut:].float(), before)
     assert len(opt.m[cut:].view(torch.uint8).unique()) > 100
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_states_that_are_refused_change_nothing(bits):
+    from fbcunn_amd import optim
+    (pf, params), (_, grads) = _tensors([300, 4097], "f32", "f32", False, 8)
+    a, b = (optim.AdamW(params, grads, stateBits=bits, **HYPER) for _ in range(2))
+    a.step(), b.step(), b.step()
+    mine = [t for t in (b.m, b.v, b.mScale, b.vScale) if t is not None]
+    before = [t.view(torch.uint8).clone() for t in mine]
+    for v, t, error in ((a.v, -1, _lib.FbfcError), (a.v[:256], 1, ValueError), ([0.0], 1, TypeError)):
+        with pytest.raises(error):
+            b.loadState(a.m, v, a.mScale, a.vScale, t)
+        assert all(torch.equal(x.view(torch.uint8), y) for x, y in zip(mine, before)) and b.t == 2
