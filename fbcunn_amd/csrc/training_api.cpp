@@ -78,9 +78,11 @@ long fbfc_adamw_state_elements(const fbfc_adamw_tensor *tensors, int count)
 static int adamw_check(const fbfc_adamw_config *c, const fbfc_adamw_tensor *tensors, int count, const void *m,
                        const void *v, const float *m_scale, const float *v_scale)
 {
-    if (c == nullptr || tensors == nullptr || m == nullptr || v == nullptr)
-        return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
+    if (c == nullptr || tensors == nullptr) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
     if (count < 1) return fail(FBFC_ERR_INVALID_ARGUMENT, "at least one tensor is needed");
+    bool empty = true;  // no parameter at all, and so no states
+    for (int i = 0; i < count; ++i) empty = empty && tensors[i].n == 0;
+    if (!empty && (m == nullptr || v == nullptr)) return fail(FBFC_ERR_INVALID_ARGUMENT, "null argument");
     if (!type_ok(c->param_type) || !type_ok(c->grad_type)) return fail(FBFC_ERR_INVALID_ARGUMENT, "unknown type");
     if (c->state_bits != 8 && c->state_bits != 32)
         return fail(FBFC_ERR_INVALID_ARGUMENT, "states have 8 or 32 bits");
@@ -88,7 +90,7 @@ static int adamw_check(const fbfc_adamw_config *c, const fbfc_adamw_tensor *tens
         return fail(FBFC_ERR_INVALID_ARGUMENT, "betas must be in [0, 1)");
     if (!(c->eps > 0 && std::isfinite(c->eps) && (float)c->eps > 0.0f))
         return fail(FBFC_ERR_INVALID_ARGUMENT, "eps must be positive");
-    if (c->state_bits == 8 && (m_scale == nullptr || v_scale == nullptr))
+    if (c->state_bits == 8 && !empty && (m_scale == nullptr || v_scale == nullptr))
         return fail(FBFC_ERR_INVALID_ARGUMENT, "states of 8 bits need their scales");
     if (!aligned(m, 16) || !aligned(v, 16)) return fail(FBFC_ERR_INVALID_ARGUMENT, "states must be 16-byte aligned");
     if (c->state_bits == 8 && (!aligned(m_scale, 4) || !aligned(v_scale, 4)))

@@ -388,3 +388,34 @@ def test_states_that_are_refused_change_nothing(bits):
         with pytest.raises(error):
             b.loadState(a.m, v, a.mScale, a.vScale, t)
         assert all(torch.equal(x.view(torch.uint8), y) for x, y in zip(mine, before)) and b.t == 2
+
+
+def test_empty_tensors_alone_need_no_states():
+    # refused for want of a GPU at most: without parameters there are no elements of states
+    for bits in (32, 8):
+        rc, message = _create_or_destroy(_config(state_bits=bits), [(0, 0, 0), (0x1000, 0, 0)], m=0, v=0, ms=0, vs=0)
+        assert rc in (_lib.OK, _lib.ERR_HIP), message
+        rc, message = _create(_config(state_bits=bits), [(0, 0, 0), (0x1000, 0x2000, 1)], m=0, v=0, ms=0, vs=0)
+        assert rc == _lib.ERR_INVALID_ARGUMENT and "null" in message
+
+
+def _create_or_destroy(config, tensors, m, v, ms, vs):
+    table = (_lib.AdamwTensor * len(tensors))(*tensors)
+    h = ctypes.c_void_p(0)
+    rc = _lib.lib().fbfc_adamw_create(ctypes.byref(config), table, len(tensors), m, v, ms, vs, ctypes.byref(h))
+    assert bool(h.value) == (rc == _lib.OK)
+    message = _lib.lib().fbfc_last_error().decode()
+    _lib.lib().fbfc_adamw_destroy(h)
+    return rc, message
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("bits", [32, 8])
+def test_steps_of_empty_tensors_are_counted(bits):
+    from fbcunn_amd import optim
+    opt = optim.AdamW([torch.zeros(0, 3, device="cuda")], [torch.zeros(0, 3, device="cuda")], stateBits=bits, **HYPER)
+    opt.step(), opt.step()
+    assert opt.t == 2 and opt.m.numel() == 0
+    opt.loadState(opt.m, opt.v, opt.mScale, opt.vScale, 7)
+    opt.step()
+    assert opt.t == 8
