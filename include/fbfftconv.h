@@ -436,8 +436,9 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_
  * for zeros.  state_out may be null, or be state_in.  The output may be one of the inputs with the same strides.
  * `lengths` (null: all of full length) holds the number of steps of each sequence, on the device, taken as between 0
  * and `steps`: what lies behind them has no effect, and the output and the gradients there are zero; state_out is the
- * state behind the last of them.  The state moves by (1 - a_t) (input_t - state), which keeps the precision of 1 - a_t; an
- * input that is infinite or NaN makes the state NaN from the next step on.  No steps or no sequences is no error: the
+ * state behind the last of them.  The state moves from the side of the larger of its two weights, by (1 - a_t) (input_t - state) or
+ * from input_t by a_t (state - input_t), so that both weights keep their precision, and behind a gate of -infinity it is the input
+ * itself.  An input that is infinite or NaN makes the state NaN, from its step or from the next on.  No steps or no sequences is no error: the
  * state passes through.  One step is the form for serving: one launch, and no workspace.  Up to 2^25 channels and 2^31
  * channels of all sequences.
  *

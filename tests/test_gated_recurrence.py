@@ -806,3 +806,60 @@ def test_parameters_that_do_not_fit_are_refused():
     net.bias.data = net.bias.data.half()       # the same tensor, of another type
     with pytest.raises(TypeError, match="bias"):
         net.updateOutput([x, gate])
+
+
+def _lerp_bound(z, x, h, new):
+    """Of one step, with z the gate: the smaller of a and 1 - a comes from e^-|z|, whose argument is rounded twice (2 |z| units),
+    with 8 units for exponential, sum, reciprocal and product; the larger is one minus that.  The state moves from the side
+    with the larger weight, so the difference's rounding counts with the smaller one."""
+    a, c = torch.sigmoid(z), torch.sigmoid(-z)
+    return U * (torch.minimum(a, c) * (2 * z.abs() + 12) * (x.abs() + h.abs()) + 2 * new.abs())
+
+
+def _large_state(B, T, dtype, order, seed):
+    """States a million times the inputs, kept as they are up to the middle, where gates from half closed to closed follow, the
+    first four closed for good; kept again behind it."""
+    net, x, gate, gy, h0, gh = _data(B, T, 60, dtype, seed, order)
+    net.bias.zero_()
+    at = T // 2
+    gate[:, :at], gate[:, at:] = float("inf"), 88.0
+    gate[:, at] = -torch.linspace(0, 40, 60, device="cuda").to(dtype)
+    gate[:, at, :4] = torch.tensor([-104.0, -300.0, torch.finfo(dtype).min, -float("inf")], device="cuda").to(dtype)
+    return net, x, gate, gy, h0 * 1e6, gh, at
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T,order", [(1, "btd"), (24, "btd"), (500, "btd"), (500, "bdt")])
+def test_a_large_state_leaves_no_rounding_behind_a_closed_gate(T, order, dtype):
+    """What is left of the state is its weight's part, and nothing rounded at the state's size; behind a gate that is closed for
+    good the state is the input itself."""
+    net, x, gate, _, h0, _, at = _large_state(3, T, TYPES[dtype], order, 28)
+    z, v, h = gate[:, at].cpu().double().clamp(min=-1000), x[:, at].cpu().double(), h0.cpu().double()
+    want = torch.sigmoid(z) * h + torch.sigmoid(-z) * v
+    bound = _lerp_bound(z, v, h, want)
+    y = net.updateOutput([x, gate], state=h0)
+    if dtype != "f16":     # 1e6 is beyond its numbers
+        _check(y[:, at], (want, bound), "output")
+    _check(net.state, (want, bound), "state")
+    assert torch.equal(y[:, at, :4], x[:, at, :4]) and torch.equal(net.state[:, :4], x[:, at, :4].float())
+    state = h0.clone()
+    token = net.step([x[:, at], gate[:, at]], state)
+    _check(state, (want, bound), "state of a token")
+    assert torch.equal(state[:, :4], x[:, at, :4].float()) and torch.equal(token[:, :4], x[:, at, :4])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", list(TYPES))
+@pytest.mark.parametrize("T,order", [(24, "btd"), (500, "btd"), (500, "bdt")])
+def test_backward_forms_the_state_behind_a_closed_gate_as_forward_does(T, order, dtype):
+    """The gate behind the closed one is half open: its gradient is u (state - x) / 4, the state the closed one's input.  u is a sum
+    of at most T + 1 numbers, rounded T times, and 12 units are left for the weights, the difference and the products."""
+    net, x, gate, gy, h0, gh, at = _large_state(3, T, TYPES[dtype], order, 29)
+    gate[:, at + 1] = 0.0
+    net.updateOutput([x, gate], state=h0)
+    net.backward([x, gate], gy, gradState=gh)
+    x, gy, gh = x.cpu().double(), gy.cpu().double(), gh.cpu().double()
+    d = x[:, at] - x[:, at + 1]
+    u, size = gh + gy[:, at + 1:].sum(1), gh.abs() + gy[:, at + 1:].abs().sum(1)
+    _check(net.gradInput[1][:, at + 1, :4], ((u * d / 4)[:, :4], (U * (T + 12) * size * d.abs() / 4)[:, :4]), "gradGate")
