@@ -85,6 +85,10 @@ class _Calls:
     def __init__(self, kind, *more):
         self._kind, self._more, self._signature, self._call, self._captured = kind, more, None, None, []
 
+    @property
+    def used(self):
+        return self._call is not None
+
     def of(self, net, inputs):
         now = signature(*inputs)
         if now != self._signature:
@@ -148,9 +152,19 @@ class GatedLinearRecurrence:
         self.gradBias = torch.zeros(nChannels, device=self.device)
         self.train = True
         self.output = self.state = self.gradInput = self.gradState = None
+        self._begin()
+
+    def _begin(self):
         self._workspace = Workspace()
         self._calls = {dims: _Calls(_RecurrenceCall, dims) for dims in (2, 3)}   # of step and updateOutput
         self._forward = None   # (shape, type, lengths, checkpoints) of the updateOutput that backward may follow
+
+    def cleanupBuffers(self):
+        """Waits for the device and gives back all memory but the last results.  No graph that was captured with the module may
+        be replayed from then on."""
+        if any(c.used for c in self._calls.values()):
+            torch.cuda.synchronize()
+        self._begin()
 
     def training(self):
         self.train = True
@@ -320,9 +334,19 @@ class GatedResidualNorm:
         self.postWeight, self.scale, self.preWeight = one(branch), one(branch), one(norm)
         self.gradPostWeight, self.gradScale, self.gradPreWeight = zero(branch), zero(branch), zero(norm)
         self.output, self.gradInput = None, None
-        self._workspace = Workspace()
         self._names = ("residual", "branch", "gate")[:1 + self.hasBranch + self.hasGate]
+        self._begin()
+
+    def _begin(self):
+        self._workspace = Workspace()
         self._calls = _Calls(_NormCall)
+
+    def cleanupBuffers(self):
+        """Waits for the device and gives back all memory but the last results.  No graph that was captured with the module may
+        be replayed from then on."""
+        if self._calls.used:
+            torch.cuda.synchronize()
+        self._begin()
 
     def parameters(self):
         pairs = [(self.postWeight, self.gradPostWeight), (self.scale, self.gradScale), (self.preWeight, self.gradPreWeight)]

@@ -863,3 +863,46 @@ def test_backward_forms_the_state_behind_a_closed_gate_as_forward_does(T, order,
     d = x[:, at] - x[:, at + 1]
     u, size = gh + gy[:, at + 1:].sum(1), gh.abs() + gy[:, at + 1:].abs().sum(1)
     _check(net.gradInput[1][:, at + 1, :4], ((u * d / 4)[:, :4], (U * (T + 12) * size * d.abs() / 4)[:, :4]), "gradGate")
+
+
+def test_buffers_of_an_unused_module_are_cleaned_up_without_a_gpu():
+    from fbcunn_amd import nn
+    for net in (nn.GatedLinearRecurrence(8, device="cpu"), nn.GatedResidualNorm(8, device="cpu")):
+        net.cleanupBuffers()
+
+
+@pytest.mark.gpu
+def test_cleanup_gives_back_what_captured_calls_took():
+    """Graphs for one length after the other: what they held goes with cleanupBuffers(), after which the module works on."""
+    net, x, gate, gy, h0, gh = _data(2, 3000, 200, torch.float32, 30)
+    other, *_ = _data(2, 3000, 200, torch.float32, 30)
+
+    def step(m, n):
+        m.updateOutput([x[:, :n], gate[:, :n]], state=h0)
+        m.backward([x[:, :n], gate[:, :n]], gy[:, :n], gradState=gh)
+
+    step(other, 3000)
+    step(net, 10)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    before = torch.cuda.memory_allocated()
+    for n in (500, 1000, 2000, 3000):
+        step(net, n)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step(net, n)
+        graph.replay()
+        torch.cuda.synchronize()
+        del graph
+    held = torch.cuda.memory_allocated()
+    last = [net.output, net.state, *net.gradInput, net.gradState]
+    net.cleanupBuffers()
+    assert all(torch.equal(a, b) for a, b in zip(last, [other.output, other.state, *other.gradInput, other.gradState]))
+    assert held - torch.cuda.memory_allocated() > 3 * sum(n * 2 * 200 * 4 for n in (500, 1000, 2000))
+    del last
+    net.output = net.state = net.gradInput = net.gradState = None
+    assert torch.cuda.memory_allocated() <= before
+    with pytest.raises(ValueError):
+        net.backward([x, gate], gy)       # follows an updateOutput
+    step(net, 3000)
+    _same(net, other, "after")

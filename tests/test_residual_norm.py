@@ -515,3 +515,17 @@ def test_parameters_that_do_not_fit_are_refused():
         setattr(net, name, whole)
     net.updateOutput(inputs)
     net.backward(inputs, grads)
+
+
+@pytest.mark.gpu
+def test_a_module_works_on_after_its_buffers_are_cleaned_up():
+    net = _net(40, "full", 1)
+    inputs, grads = _inputs((70, 40), "full", torch.float32, 10)
+    want = [t.clone() for t in net.updateOutput(inputs) + net.backward(inputs, grads) + net.parameters()[1]]
+    assert len(net._workspace._of) == 1
+    net.cleanupBuffers()
+    assert not net._workspace._of
+    for t in net.parameters()[1]:
+        t.fill_(float("nan"))
+    for a, b in zip(want, net.updateOutput(inputs) + net.backward(inputs, grads) + net.parameters()[1]):
+        assert torch.equal(a, b)
