@@ -290,8 +290,8 @@ __device__ __forceinline__ float open_of(float m) { return holds_a(m) ? -m : 1.0
 // v a, rounded once
 __device__ __forceinline__ float kept(float m, float v) { return fmaf(-m, v, holds_a(m) ? 0.0f : v); }
 // The state after h and x, which are `d` = x - h apart, from the side of the larger weight: h + (1 - a) d or x - a d.  So behind a
-// closed gate it is x, with no rounding of the size of h.  With h + (1 - a) d alone a step has 7 operations less, and 8 sequences
-// of 2048 steps x 1024 channels in bf16 take 28.8 us forward instead of 29.5, 131072 steps x 2048 channels 1048 us in training instead of 1063.
+// closed gate it is x, with no rounding of the size of h.  (With h + (1 - a) d alone, and a (1 - (1 - a)) in products: 8 sequences of
+// 2048 steps x 1024 channels in bf16 forward 28.7 us, 29.7 so; 131072 steps x 2048 channels 1047 us in training, 1055 so.)
 __device__ __forceinline__ float moved(float m, float h, float x, float d) { return fmaf(m, d, holds_a(m) ? x : h); }
 
 // Tickets count the tiles of all columns (sequences and blocks of channels) in the order in which they depend on each
@@ -414,40 +414,37 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
         const long t0 = ((long)__builtin_amdgcn_readfirstlane(tile) * s.waves + w) * kRun;
         const int n = steps_before(t0, len), n_all = steps_before(t0, steps);
         const bool full = n == kRun && whole;
-        // m: the gates, kept for the second way through the steps: evaluated again, the two gates a lane cost more than their
-        // registers do (131072 steps of 2048 channels in bf16: 385 us so, 372 us kept).
-        Vec<T, V> x[kRun];
-        float m[kRun][V], A[V], S[V];
-#pragma unroll
-        for (int i = 0; i < V; ++i) {
-            A[i] = 1.0f;
-            S[i] = 0.0f;
-#pragma unroll
-            for (int t = 0; t < kRun; ++t) m[t][i] = 0.0f;
-        }
+        // The runs from the wavefront's first step to each of its steps, so that one operation a step is left once the state
+        // before them is known (131072 steps of 2048 channels in bf16: 384 us so, 391 with the gates kept in their place).
+        float A[kRun][V], S[kRun][V];
         auto read = [&](auto all) {
             constexpr bool FULL = decltype(all)::value;
-            Vec<T, V> gate[kRun];
+            Vec<T, V> x[kRun], gate[kRun];
             xr.template load<FULL>(x, t0, n, len, c, a.channels);
             gr.template load<FULL>(gate, t0, n, len, c, a.channels);
-            if (!FULL && n < kRun) cut_run<T, V>(x, n);
 #pragma unroll
             for (int t = 0; t < kRun; ++t) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    if (FULL || t < n) m[t][i] = gate_of((float)gate[t][i], bias2[i]);
-                    A[i] = kept(m[t][i], A[i]);
-                    S[i] = moved(m[t][i], S[i], (float)x[t][i], (float)x[t][i] - S[i]);
+                    const float a = t > 0 ? A[t > 0 ? t - 1 : 0][i] : 1.0f, h = t > 0 ? S[t > 0 ? t - 1 : 0][i] : 0.0f;
+                    const float m = gate_of((float)gate[t][i], bias2[i]), xt = (float)x[t][i];
+                    A[t][i] = FULL || t < n ? kept(m, a) : a;
+                    S[t][i] = FULL || t < n ? moved(m, h, xt, xt - h) : h;
                 }
                 if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
         };
         if (full) read(std::true_type{});
         else if (len > 0) read(std::false_type{});
+        else
+#pragma unroll
+            for (int t = 0; t < kRun; ++t)
+#pragma unroll
+                for (int i = 0; i < V; ++i) A[t][i] = 1.0f, S[t][i] = 0.0f;
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            sA[turn][w][lane * V + i] = A[i];
-            sS[turn][w][lane * V + i] = S[i];
+            sA[turn][w][lane * V + i] = A[kRun - 1][i];
+            sS[turn][w][lane * V + i] = S[kRun - 1][i];
         }
         __syncthreads();
         // the runs of the wavefronts before this one, as one; of the whole tile in the first wavefront
@@ -473,11 +470,9 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
             }
         }
         __syncthreads();
-        float h[V];
+        float h[V];  // the state before the wavefront's steps
 #pragma unroll
         for (int i = 0; i < V; ++i) h[i] = fmaf(Ap[i], carried[lane * V + i], Sp[i]);
-#pragma unroll
-        for (int t = 0; t < kRun; ++t) forget<T, V>(x[t]);
         auto write = [&](auto all) {
             constexpr bool FULL = decltype(all)::value;
             const char *to = yr.row(t0);
@@ -485,10 +480,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
             for (int t = 0; t < kRun; ++t, to += yr.st) {
                 float out[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    if (FULL || t < n) h[i] = moved(m[t][i], h[i], (float)x[t][i], (float)x[t][i] - h[i]);
-                    out[i] = FULL || t < n ? h[i] : 0.0f;
-                }
+                for (int i = 0; i < V; ++i) out[i] = FULL || t < n ? fmaf(A[t][i], h[i], S[t][i]) : 0.0f;
                 if (FULL || t < n_all) yr.template store<FULL>(to, c, a.channels, out);
                 if (t % 2 == 1) __builtin_amdgcn_sched_barrier(0);
             }
@@ -498,7 +490,7 @@ __global__ __launch_bounds__(kLanes *kWaves, 4) void recurrence_forward_kernel(R
         if (a.state_out != nullptr && tile + 1 == s.tiles && w + 1 == s.waves)
 #pragma unroll
             for (int i = 0; i < V; ++i)
-                if (c + i < a.channels) a.state_out[(long)b * a.channels + c + i] = h[i];
+                if (c + i < a.channels) a.state_out[(long)b * a.channels + c + i] = fmaf(A[kRun - 1][i], h[i], S[kRun - 1][i]);
     }
 }
 
