@@ -4,7 +4,8 @@
 //   p = p (1 - lr decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
 //
 // in 32 bits, every operation rounded by itself (this file is compiled without contraction of a product and a sum),
-// so that a plain evaluation of the formulas gives the same states bit for bit.
+// so that a plain evaluation of the formulas gives the same states bit for bit, and with 32-bit states the same parameters.
+// With 8-bit states the parameter's quotient takes a root and a reciprocal that are off by up to one unit each.
 //
 // The step is bound by memory: 28 bytes a parameter in 32 bits, 14 with 32-bit parameters, 16-bit gradients and
 // 8-bit states.  One launch takes all tensors: a table of pieces of 4096 parameters, walked by at most 2048 workgroups,

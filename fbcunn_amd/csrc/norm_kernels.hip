@@ -12,14 +12,17 @@
 // Everything in a row is in 32 bits and rounded once where it is stored; n is the norm of r' before that rounding, and
 // the backward pass computes r' again from its inputs (it would have to read r' otherwise, as many bytes).
 //
-// Bound by memory: a forward pass reads three rows and writes two, a backward pass reads five and writes three.  A row
-// stays in registers from its first load to its last store, with all its loads issued before the first sum.  Rows of up
+// Bound by memory: a forward pass reads three rows and writes two, a backward pass reads five and writes three.  A row of
+// up to 8192 channels stays in registers from its first load to its last store, with all its loads issued before the first sum.
+// Longer ones take a workgroup of more than 512 threads, whose 128 registers do not hold it: forward in 32 bits, and backward in
+// every type, part of it goes through scratch memory (4096 rows of 12288 channels: forward 101 us in bf16, 472 us (2.1 TB/s) in
+// 32 bits; backward 644 us (1.3 TB/s) in bf16, 1033 us in 32 bits; of 8192 channels 67, 129, 149 and 227 us).  Rows of up
 // to 1024 channels take 8 to 64 lanes, and longer ones a workgroup, whose wavefronts exchange their sums through
 // the LDS with one barrier a sum.  The workgroups walk over the rows, so that the weights and the sums of the weights'
 // gradients stay in registers too; these are then added over the workgroups in a fixed order by a second kernel.
 //
 // Measured: 8192 rows of 2048 channels in bf16 forward 35.9 us (4.67 TB/s; a copy of that size reaches 5.5); 65536 rows of
-// 4096 in bf16 backward 871 us (4.93 TB/s, what a large copy reaches); 3001 rows of 1000 in 32 bits backward 25 us and 4.6 us
+// 4096 in bf16 backward 871 us (4.93 TB/s, what a large copy reaches); 3001 rows of 1000 in 32 bits backward 25 us and 4.7 us
 // for the sums of the weights' gradients.
 #include <hip/hip_runtime.h>
 
@@ -209,7 +212,7 @@ __global__ __launch_bounds__(most_threads(L)) void norm_backward_kernel(NormArgs
     __shared__ float slot[4][kMaxWaves];
     const RowWalk<L> walk;
     const bool branch = a.branch.data != nullptr, gated = a.gate.data != nullptr, normed = a.grad_normed.data != nullptr;
-    // with 128 registers there are none for the weights: read again for each row, from the caches
+    // with 128 registers, which the row itself passes already, the weights are read again for each row, from the caches
     constexpr bool kKeep = L != kWidest;
     int c[E];
     float post[N], pre[N], q[N], s[N];

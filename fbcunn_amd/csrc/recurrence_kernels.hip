@@ -19,9 +19,9 @@
 // Backward does the same from the last tile to the first; the states h inside a tile come from the state before it, which
 // the forward pass leaves in `checkpoints` (4 bytes for 128 steps), so y is neither read nor relied on to have 32 bits.
 //
-// Measured: 131072 steps of 2048 channels in bf16, forward 372 us (4.3 TB/s), backward 657 us (4.1 TB/s; a large copy
-// reaches 5.0 TB/s); without the walk back the forward pass would take 287 us.  8 sequences of 2048 steps x 1024 channels in bf16
-// forward 26.8 us (3.8 TB/s) and 2 to 4.6 us for clearing: its 1024 workgroups begin in step and read and write by turns.
+// Measured: 131072 steps of 2048 channels in bf16, forward 384 us (4.2 TB/s), backward 661 us (4.1 TB/s; a large copy
+// reaches 5.0 TB/s); without the walk back the forward pass took 287 us where it takes 372 with it.  8 sequences of 2048 steps x
+// 1024 channels in bf16 forward 28 us (3.6 TB/s) and 2 to 4.6 us for clearing: its 1024 workgroups begin in step and read and write by turns.
 #include <hip/hip_runtime.h>
 
 #include <type_traits>

@@ -350,7 +350,7 @@ enum { FBFC_F32 = 0, FBFC_BF16 = 1, FBFC_F16 = 2 };
  *     g' = grad_scale g        m = beta1 m + (1 - beta1) g'        v = beta2 v + (1 - beta2) g'^2
  *     p = p (1 - lr weight_decay) - lr / (1 - beta1^t) * m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
  * in 32 bits, t = 1 at the first step; p is rounded to the nearest of its type, so a parameter of 16 bits does not
- * notice a step below half its spacing.
+ * notice a step below half its spacing.  With 8-bit states the root and the quotient are off by up to a unit of 32 bits each.
  *
  * The optimizer holds the addresses of the parameters and of their gradients (which the layers keep in place) and the
  * number of steps; the states belong to the caller, one array each for m and v, in which every tensor begins at a
@@ -433,7 +433,8 @@ int fbfc_residual_norm_backward(const fbfc_residual_norm_desc *desc, const fbfc_
  * Element (b, t, c) of a tensor lies b * stride_batch + t * stride_step + c * stride_channel values from `data`, any
  * strides for what is read; channels side by side (stride_channel 1) are the fast order, steps side by side, as in the
  * planes of a convolution, are supported.  gate_bias has `channels` values, the states (batch, channels); null stands
- * for zeros.  state_out may be null, or be state_in.  The output may be one of the inputs with the same strides.
+ * for zeros.  state_out may be null, or be state_in.  The output may be one of the inputs with the same strides.  But for
+ * these, and grad_state_in below, nothing that is written may overlap anything.
  * `lengths` (null: all of full length) holds the number of steps of each sequence, on the device, taken as between 0
  * and `steps`: what lies behind them has no effect, and the output and the gradients there are zero; state_out is the
  * state behind the last of them.  The state moves from the side of the larger of its two weights, by (1 - a_t) (input_t - state) or
