@@ -213,7 +213,7 @@ class GatedLinearRecurrence:
         call, places, stream = self._call(input, 3)
         bias = _parameter(self.bias, "bias", self.nChannels, call.index)
         first, sizes = self._check_state(state, "state", call), self._check_lengths(lengths, call)
-        self.output = call.result(0, places)
+        self.output = call.result(0, places + (first or 0,))
         self.state = call.result(3, places)
         kept = call.result(5) if self.train else None
         call.steps[2].data = self.output.data_ptr()

@@ -906,3 +906,25 @@ def test_cleanup_gives_back_what_captured_calls_took():
         net.backward([x, gate], gy)       # follows an updateOutput
     step(net, 3000)
     _same(net, other, "after")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("T", [1, 40, 700])
+def test_a_state_that_is_a_row_of_the_own_output_keeps_its_values(T):
+    """One sequence in parts, each from the last output of the part before, which is needed again."""
+    net, x, gate, gy, h0, _ = _data(1, T, 40, torch.float32, 31)
+    other, *_ = _data(1, T, 40, torch.float32, 31)
+    first = net.updateOutput([x, gate], state=h0)
+    kept = first.clone()
+    net.updateOutput([x, gate], state=first[:, -1])
+    other.updateOutput([x, gate], state=kept[:, -1])
+    assert torch.equal(first, kept)
+    net.backward([x, gate], gy, gradState=first[:, 0])
+    other.backward([x, gate], gy, gradState=kept[:, 0])
+    _same(net, other, "output")
+    first = net.gradInput[0]
+    kept = first.clone()
+    net.backward([x, gate], gy, gradState=first[:, 0])
+    other.backward([x, gate], gy, gradState=kept[:, 0])
+    assert torch.equal(first, kept)
+    _same(net, other, "gradInput")
