@@ -185,11 +185,11 @@ __device__ __forceinline__ void announce_state(const Chain &ch, const Shape &s, 
 // or before a lane, its loads are moved back to end with the row, so that no load has a condition, and an odd last channel
 // is then moved to its place.  Orders of memory: kDense, channels side by side, with an offset that fits 32 bits, so that the
 // row's address stays in scalar registers; kPlanes, steps side by side, as a convolution leaves them: each lane reads its 16
-// steps in vectors of 16 bytes (8 sequences of 2048 steps x 1024 channels in 32 bits, input and gate in planes, forward 42 us so, 76
-// one step at a time; 38 with the channels side by side; in bf16 28.5, 77 and 28); kAny.
+// steps in vectors of 16 bytes (8 sequences of 2048 steps x 1024 channels in 32 bits, input and gate in planes, forward 43 us so, 76
+// one step at a time; 38 with the channels side by side; in bf16 29, 77 and 29); kAny.
 //
 // Forward, a lane has 4 bytes of each row, two channels in 16 bits.  Backward it has one: with two, a wavefront needs 178
-// registers instead of 111, and one workgroup fits a CU where two do (131072 steps of 2048 channels in bf16: 752 us with two
+// registers instead of 113, and one workgroup fits a CU where two do (131072 steps of 2048 channels in bf16: 752 us with two
 // channels, 662 with one; forward 393 with two and 425 with one).
 enum Order { kAny, kDense, kPlanes };
 template <typename T, Order IN>
